@@ -476,6 +476,94 @@ KCG_API int kcg_layernorm_allgather_multicast(int dtype, int64_t rows, int64_t c
                                               void* stream);
 
 /*
+ * Paged 8-bit key / value cache (no counterpart in the reference, whose attention reads dense
+ * tensors of one length, src/Optimizer/Optimizer.cc:2606-2860).
+ *
+ * The cache is a pool of num_pages pages of page_size tokens each.  k_cache and v_cache hold e4m3
+ * codes, addressed as base + page*stride[0] + head*stride[1] + row*stride[2] + d (bytes), so that
+ * [pages, Hkv, page_size, D] and [pages, page_size, Hkv, D] are both expressible; k_scale and
+ * v_scale are fp32 [pages, Hkv]; a stored value is code * scale.  Row i of block_table (int32,
+ * table_width entries, rows table_stride apart) lists the pages of request i in order: its token p
+ * lives in page block_table[i][p / page_size], row p % page_size, and that place's number,
+ * page * page_size + row, is the token's slot.
+ *
+ * kcg_cache_plan prepares a step in which request i, with cached[i] tokens in the cache, adds
+ * fresh[i]:
+ *   - the pages it needs beyond those it has are taken from the end of free_pages[0 .. *free_count)
+ *     (a stack), request after request, and entered in block_table; other entries stay as they are;
+ *   - slot_map[t] is the slot of token t of the step, the tokens of request 0 first; entries behind
+ *     the last token, up to max_tokens, are -1;
+ *   - cu_new[0 .. requests] are the prefix sums of `fresh` (cut at max_tokens), lengths[i] =
+ *     cached[i] + fresh[i], and *free_left the number of pages left.
+ * A request is served when the pages wanted up to and with it do not exceed *free_count (or it wants
+ * none), its tokens end at or before max_tokens and its table row is wide enough.  One that is not
+ * served changes nothing: lengths[i] = cached[i], its tokens' slots are -1, and its share of pages
+ * stays free.  Negative counts and a *free_count outside [0, free_capacity] are reported by
+ * kcg_device_status() (KCG_ERR_INVALID_ARG); such a request is not served, the count is clamped.
+ * lengths may be cached and free_left may be free_count (update in place); slot_map and
+ * block_table overlap nothing.  At most 16384 requests.
+ */
+KCG_API int kcg_cache_plan(int64_t requests, int64_t page_size, int64_t max_tokens,
+                           const int32_t* cached, const int32_t* fresh, int32_t* block_table,
+                           int64_t table_width, int64_t table_stride, const int32_t* free_pages,
+                           int64_t free_capacity, const int32_t* free_count, int32_t* lengths,
+                           int32_t* cu_new, int64_t* slot_map, int32_t* free_left, void* stream);
+
+/*
+ * Writes token t's keys and values, K and V [T, Hkv, D] (element strides of token and head; D
+ * contiguous), into slot slot_map[t].  Slots of -1 are skipped; others outside the pool are skipped
+ * too and reported by kcg_device_status() (KCG_ERR_INVALID_ARG).
+ *
+ * Scale of a page and head: the smallest power of two s with amax / s <= 448 (at least 2^-110),
+ * amax the largest finite magnitude this call writes there.  Tokens that begin at a page's first row
+ * start it anew; otherwise the page keeps max(s, its scale), and where that grows its rows before the
+ * first one written are rounded again.  Rows behind the written ones keep their bytes.  Infinities
+ * and NaN are stored as NaN (e4m3 has no infinity).
+ * The tokens of one page must stand together in slot_map, in ascending slots (as kcg_cache_plan
+ * orders them), with at most 31 skipped tokens between two of them; a page that breaks this, or a
+ * slot that occurs twice, leaves that page's contents (and no other's) unspecified.
+ *
+ * dtype of K and V: KCG_BF16, KCG_F16 or KCG_F32; D in {64, 128}; page_size a multiple of 16; rows
+ * of K, V and the caches start on 16-byte boundaries.
+ */
+KCG_API int kcg_cache_append(int dtype, int64_t T, int64_t Hkv, int64_t D, const void* K,
+                             const int64_t k_strides[2], const void* V, const int64_t v_strides[2],
+                             const int64_t* slot_map, int64_t num_pages, int64_t page_size,
+                             void* k_cache, const int64_t kc_strides[3], void* v_cache,
+                             const int64_t vc_strides[3], float* k_scale, float* v_scale,
+                             void* stream);
+
+/*
+ * Attention forward of new tokens over the cache that already holds them.  Request i has the rows
+ * [cu_new[i], cu_new[i+1]) of Q [T, Hq, D] and O (cu_new == NULL: T / B rows each) and lengths[i]
+ * tokens in the cache, its new ones last; query head h uses key head h / (Hq / Hkv):
+ *   O[j,h,:] = sum_t softmax_t(softmax_scale * Q[j,h,:].K[t,:]) * V[t,:],  t < lengths[i];
+ *   causal != 0 masks t > lengths[i] - n + j for the request's j-th of n rows (kcg_fmha_fwd's mask).
+ * Rows that see no key are zero; rows of O outside [cu_new[0], cu_new[B]) stay as they were.  Nothing
+ * is read behind a request's last token.  Block table entries outside the pool are not followed:
+ * their keys are left out, and kcg_device_status() reports KCG_ERR_INVALID_ARG, as it does for
+ * lengths beyond the table (cut) and a cu_new that descends or leaves [0, T] (clamped).
+ * max_new: the most rows a request has, as far as the caller knows (0: T); it chooses the kernel, and
+ * a wrong value costs time only.
+ *
+ * dtype of Q and O: KCG_BF16 or KCG_F16; D in {64, 128}; page_size a multiple of 16; any fp32
+ * scales.  Statistics and sums are fp32, P is rounded to fp16.
+ * `workspace`: kcg_fmha_cached_workspace bytes of the current device, 16-byte aligned, for this call
+ * alone until it has run; its contents need not be kept or cleared.
+ */
+KCG_API int kcg_fmha_cached_workspace(int64_t D, size_t* bytes);
+KCG_API int kcg_fmha_cached_fwd(int dtype, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                int64_t max_new, float softmax_scale, int causal, const void* Q,
+                                const int64_t q_strides[2], const void* k_cache,
+                                const int64_t kc_strides[3], const float* k_scale,
+                                const void* v_cache, const int64_t vc_strides[3],
+                                const float* v_scale, int64_t num_pages, int64_t page_size,
+                                const int32_t* block_table, int64_t table_width,
+                                int64_t table_stride, const int32_t* lengths,
+                                const int32_t* cu_new, void* O, const int64_t o_strides[2],
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Device memory that other processes on the node can map (CUDA IPC).  kcg_peer_alloc returns a
  * plain device allocation; kcg_peer_export fills a 64-byte handle that another process passes
  * to kcg_peer_open to obtain a pointer valid on its own GPU (peer access is enabled on first

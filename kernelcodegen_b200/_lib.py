@@ -63,6 +63,12 @@ SIGNATURES = {
     "kcg_fmha_fwd_allgather": ([_ci, _i64, _i64, _i64, _i64, _i64, _fp, _ci, _vp, _i64p, _vp, _i64p, _vp, _i64p,
                                 ctypes.POINTER(_vp), _ci, _ci, _i64, _i64p, _vp], _ci),
     "kcg_fmha_set_p_in_tmem": ([_ci], None),
+    "kcg_cache_plan": ([_i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp], _ci),
+    "kcg_cache_append": ([_ci, _i64, _i64, _i64, _vp, _i64p, _vp, _i64p, _vp, _i64, _i64, _vp, _i64p, _vp, _i64p, _vp, _vp,
+                          _vp], _ci),
+    "kcg_fmha_cached_workspace": ([_i64, ctypes.POINTER(ctypes.c_size_t)], _ci),
+    "kcg_fmha_cached_fwd": ([_ci, _i64, _i64, _i64, _i64, _i64, _i64, _fp, _ci, _vp, _i64p, _vp, _i64p, _vp, _vp, _i64p,
+                             _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64p, _vp, ctypes.c_size_t, _vp], _ci),
     "kcg_gather": ([_ci, _ci, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp], _ci),
     "kcg_transpose": ([_ci, _i64, _i64, _i64, _vp, _vp, _vp], _ci),
     "kcg_device_count": ([ctypes.POINTER(_ci)], _ci),

@@ -5,7 +5,8 @@ Names and argument meaning follow the reference's operator builders
 (BatchedMatmul with Layout flags), ``softmax``, ``layernorm`` (axis, eps), ``elementwise``
 ("Tanh" | "Sqrt" | "Log" | "Relu" | "Cast" | "Gelu"), ``relu``, ``binary`` ("Add" | "Mul" |
 "Div" | "Sub" | "Pow" | "Equal" | "Greater"), ``gather``, ``transpose`` and ``fmha`` for the
-fused BatchedMatmul -> Softmax -> BatchedMatmul chain.  torch only supplies device memory and
+fused BatchedMatmul -> Softmax -> BatchedMatmul chain.  ``cache_plan``, ``cache_append`` and
+``fmha_cached`` serve a paged 8-bit key / value cache.  torch only supplies device memory and
 the current stream; every computation is a call through the C ABI into the sm_100a
 kernels, and there is no fallback path.
 """
@@ -362,4 +363,192 @@ def fmha(Q, K, V, softmax_scale: float = 1.0, causal: bool = False, out_layout: 
     check(_lib.load().kcg_fmha_fwd(_dt(Q), B, H, Sq, Skv, D, float(softmax_scale), int(causal),
                                    Q.data_ptr(), st(Q), K.data_ptr(), st(K), V.data_ptr(), st(V),
                                    out.data_ptr(), st(out), _stream()), "kcg_fmha_fwd")
+    return out
+
+
+# ---- paged 8-bit key / value cache ------------------------------------------------------------------
+# k_cache / v_cache: float8_e4m3fn [pages, Hkv, page_size, D] (any strides with D contiguous, e.g. a
+# [pages, page_size, Hkv, D] buffer seen through a permutation); k_scale / v_scale: float32 [pages, Hkv];
+# row i of block_table lists the pages of request i in order.
+
+_workspace_bytes: dict = {}
+
+
+class _On:
+    """Makes a tensor's device current for a launch, when it is not the current one already."""
+    __slots__ = ("guard",)
+
+    def __init__(self, t):
+        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _vector(what: str, name: str, t, dtype, n=None) -> None:
+    if t.dim() != 1 or t.dtype != dtype or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{what}: {name} must be a contiguous {dtype} vector" + ("" if n is None else f" of {n}"))
+
+
+def _outer_strides(t):
+    """Strides of all dims but the last; of a dim with one entry (or none) any stride will do: 0."""
+    return _i64arr([s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride())])
+
+
+def _no_overlap(what: str, name: str, t) -> None:
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"{what}: {name} is written and must not be an expanded view")
+
+
+def _check_table(what: str, table, requests: int) -> None:
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] < requests:
+        raise ValueError(f"{what}: block_table must be an int32 matrix with a row for each of {requests} requests")
+    if table.shape[1] > 1 and table.stride(1) != 1 or table.shape[0] > 1 and table.stride(0) < table.shape[1]:
+        raise ValueError(f"{what}: the rows of block_table must be contiguous and apart from each other")
+
+
+def _check_cache(what: str, k_cache, v_cache, k_scale, v_scale) -> None:
+    shape = k_cache.shape
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        if t.dim() != 4 or t.dtype != torch.float8_e4m3fn or t.shape != shape or t.stride(3) != 1:
+            raise ValueError(f"{what}: {name} must be float8_e4m3fn [pages, Hkv, page_size, D] with a contiguous last dim, "
+                             "k_cache and v_cache of one shape")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t.dtype != torch.float32 or t.shape != shape[:2] or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous float32 [pages, Hkv]")
+
+
+def _one_device(what: str, first, *ts) -> None:
+    if not first.is_cuda:
+        raise ValueError("operands must be CUDA tensors (there is no CPU path)")
+    for t in ts:
+        if t.device != first.device:
+            raise ValueError(f"{what}: operands are on {first.device} and {t.device}")
+
+
+def cache_plan(cached, new, block_table, free_pages, free_count, page_size: int, max_tokens: int, out=None):
+    """A step's pages and slots from request lengths, on the GPU.
+
+    ``cached`` and ``new`` (int32 [B]) are each request's tokens in the cache and tokens to add.  Pages a
+    request needs beyond those it has are taken from the end of ``free_pages[:free_count]`` (int32 list,
+    int32 [1] count), request after request, and entered in ``block_table`` (int32 [>= B, width], updated in
+    place).  Returns ``(lengths, cu_new, slot_map, free_left)``: int32 [B] lengths after the step, int32 [B + 1]
+    prefix sums of ``new``, int64 [max_tokens] slots (-1 behind the last token) and the int32 [1] count of
+    pages left.  ``out`` may name those four tensors; ``lengths`` may be ``cached`` and ``free_left`` may be
+    ``free_count``.  A request that cannot be given all of its pages (or whose tokens end behind max_tokens, or
+    whose table row is too short) is left as it was: lengths[i] == cached[i], slots -1.  ``block_table`` may
+    have more rows than there are requests; those behind the last one are not touched."""
+    what = "cache_plan"
+    _vector(what, "cached", cached, torch.int32)
+    B = cached.shape[0]
+    _vector(what, "new", new, torch.int32, B)
+    _check_table(what, block_table, B)
+    _vector(what, "free_pages", free_pages, torch.int32)
+    _vector(what, "free_count", free_count, torch.int32, 1)
+    if max_tokens < 0 or page_size < 1:
+        raise ValueError("cache_plan: max_tokens and page_size must not be negative or zero")
+    _one_device(what, cached, new, block_table, free_pages, free_count)
+    if out is None:
+        dev = cached.device
+        lengths = torch.empty(B, dtype=torch.int32, device=dev)
+        cu_new = torch.empty(B + 1, dtype=torch.int32, device=dev)
+        slot_map = torch.empty(max_tokens, dtype=torch.int64, device=dev)
+        free_left = torch.empty(1, dtype=torch.int32, device=dev)
+    else:
+        lengths, cu_new, slot_map, free_left = out
+        _vector(what, "out lengths", lengths, torch.int32, B)
+        _vector(what, "out cu_new", cu_new, torch.int32, B + 1)
+        _vector(what, "out slot_map", slot_map, torch.int64, max_tokens)
+        _vector(what, "out free_left", free_left, torch.int32, 1)
+        _one_device(what, cached, lengths, cu_new, slot_map, free_left)
+    with _On(cached):
+        check(_lib.load().kcg_cache_plan(B, page_size, max_tokens, cached.data_ptr(), new.data_ptr(),
+                                         block_table.data_ptr(), block_table.shape[1],
+                                         max(block_table.stride(0), block_table.shape[1]), free_pages.data_ptr(),
+                                         free_pages.shape[0], free_count.data_ptr(), lengths.data_ptr(),
+                                         cu_new.data_ptr(), slot_map.data_ptr(), free_left.data_ptr(), _stream()),
+              "kcg_cache_plan")
+    return lengths, cu_new, slot_map, free_left
+
+
+def cache_append(K, V, slot_map, k_cache, v_cache, k_scale, v_scale) -> None:
+    """Writes keys and values of new tokens (K, V [T, Hkv, D], 16-bit or float32, D contiguous) into the slots
+    ``slot_map`` (int64 [T]; -1 skips a token) names, as e4m3 codes with one power-of-two scale per page and
+    head.  A page that already holds tokens keeps the larger scale, and its older rows are rounded again where
+    it grows.  The tokens of a page stand together in ``slot_map``, ascending, as ``cache_plan`` orders them, with
+    at most 31 skipped ones between two; otherwise the contents of that page are unspecified."""
+    what = "cache_append"
+    _check_cache(what, k_cache, v_cache, k_scale, v_scale)
+    pages, Hkv, page_size, D = k_cache.shape
+    for name, t in (("K", K), ("V", V)):
+        if t.dim() != 3 or t.shape != K.shape or tuple(t.shape[1:]) != (Hkv, D) or t.stride(2) != 1:
+            raise ValueError(f"{what}: {name} must be [T, {Hkv}, {D}] with a contiguous last dim, K and V of one shape")
+    _same_dtype(what, K, V)
+    _no_overlap(what, "k_cache", k_cache)
+    _no_overlap(what, "v_cache", v_cache)
+    _vector(what, "slot_map", slot_map, torch.int64, K.shape[0])
+    _one_device(what, K, V, slot_map, k_cache, v_cache, k_scale, v_scale)
+    with _On(K):
+        check(_lib.load().kcg_cache_append(_dt(K), K.shape[0], Hkv, D, K.data_ptr(), _outer_strides(K), V.data_ptr(),
+                                           _outer_strides(V), slot_map.data_ptr(), pages, page_size,
+                                           k_cache.data_ptr(), _outer_strides(k_cache), v_cache.data_ptr(),
+                                           _outer_strides(v_cache), k_scale.data_ptr(), v_scale.data_ptr(),
+                                           _stream()), "kcg_cache_append")
+
+
+def fmha_cached(Q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, cu_new=None, softmax_scale: float = 1.0,
+                causal: bool = False, max_new: int = 0, out=None):
+    """Attention of new tokens over the paged cache that already holds them: ``fmha`` for requests of
+    different lengths, with key / value heads shared by groups of query heads.
+
+    Q [T, Hq, D] packs the requests' rows one after another; ``cu_new`` (int32 [B + 1], from ``cache_plan``)
+    says where each begins, or None when all have T / B.  ``lengths`` (int32 [B]) counts a request's tokens in
+    the cache, the new ones last; causal masks keys behind a row's own.  Returns O like Q; rows that see no
+    key are zero, rows outside cu_new's range are left as they were in ``out`` (unspecified without ``out``).
+    ``max_new``: the most rows one request has, if the caller knows it; it only chooses the kernel."""
+    what = "fmha_cached"
+    _check_cache(what, k_cache, v_cache, k_scale, v_scale)
+    pages, Hkv, page_size, D = k_cache.shape
+    if Q.dim() != 3 or Q.shape[2] != D or Q.stride(2) != 1:
+        raise ValueError(f"{what}: Q must be [T, Hq, {D}] with a contiguous last dim")
+    T, Hq, _ = Q.shape
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"{what}: {Hq} query heads do not divide into {Hkv} key heads")
+    _vector(what, "lengths", lengths, torch.int32)
+    B = lengths.shape[0]
+    _check_table(what, block_table, B)
+    if cu_new is not None:
+        _vector(what, "cu_new", cu_new, torch.int32, B + 1)
+    elif B == 0 or T % B:
+        raise ValueError(f"{what}: without cu_new, {T} rows must divide into {B} requests")
+    _one_device(what, Q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, *(() if cu_new is None else (cu_new,)))
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=Q.dtype, device=Q.device)
+    elif out.shape != Q.shape or out.dtype != Q.dtype or out.device != Q.device or out.stride(2) != 1:
+        raise ValueError(f"{what}: out must be a {tuple(Q.shape)} {Q.dtype} tensor on {Q.device} with a contiguous last dim")
+    else:
+        _no_overlap(what, "out", out)
+    with _On(Q):
+        lib = _lib.load()
+        key = (Q.device.index, D)
+        nbytes = _workspace_bytes.get(key)
+        if nbytes is None:
+            size = ctypes.c_size_t()
+            check(lib.kcg_fmha_cached_workspace(D, ctypes.byref(size)), "kcg_fmha_cached_workspace")
+            nbytes = _workspace_bytes[key] = size.value
+        # from the caching allocator, on the launching stream: calls on other streams get memory of their own
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
+        check(lib.kcg_fmha_cached_fwd(_dt(Q), T, B, Hq, Hkv, D, max_new, float(softmax_scale), int(causal), Q.data_ptr(),
+                                      _outer_strides(Q), k_cache.data_ptr(), _outer_strides(k_cache),
+                                      k_scale.data_ptr(), v_cache.data_ptr(), _outer_strides(v_cache),
+                                      v_scale.data_ptr(), pages, page_size, block_table.data_ptr(), block_table.shape[1],
+                                      max(block_table.stride(0), block_table.shape[1]), lengths.data_ptr(),
+                                      None if cu_new is None else cu_new.data_ptr(), out.data_ptr(),
+                                      _outer_strides(out), workspace.data_ptr(), nbytes, _stream()),
+              "kcg_fmha_cached_fwd")
     return out
