@@ -8,15 +8,15 @@
 //
 // `cached_split_kernel` serves few query rows per request (decoding).  There the cost is reading the cache:
 // 2 L D bytes per key / value head, each read once and used for the G query heads of its group.
-//   - The G heads and n_i queries of a key / value head share its keys as the rows of one 16-row tile, so a byte
-//     is loaded and converted once.  Products run on mma.sync m16n8k16: at 16 rows a 128-row tcgen05 tile would be
-//     seven eighths padding, and tensor time is not what bounds this kernel.
+//   - The G heads and n_i queries of a key / value head share its keys as the columns of one tile of 8 NQ rows of Q,
+//     so a byte is loaded and converted once.  Products run on mma.sync m16n8k16 with the cache as the 16-row
+//     operand (S^T = K Q^T, O^T = V^T P^T): eight query rows cost no padding, where a tcgen05 tile would want 128.
 //   - Work is cut in units of 128 keys of one (request, head, 16 rows); the units of the whole batch, numbered in
 //     that order, are dealt to a fixed grid in equal contiguous ranges, whatever the lengths: every block finds its
 //     range by a prefix sum over the requests.  A block leaves a partial result (running maximum, sum, output) for
 //     at most its first and its last item; cached_join_kernel merges those in a fixed order.
-//   - A warp owns 32 keys of a unit and a ring of its own in shared memory, filled by cp.async two tiles ahead,
-//     across item borders; no block barrier stands in the loop.  Masked rows are not loaded but zero-filled.
+//   - A warp owns 32 keys of a unit and a ring of its own in shared memory, which one of its lanes fills by TMA
+//     (boxes of 16 or 32 rows of a page) ahead of use and across item borders; no block barrier stands in the loop.
 //   - Codes become f16 in registers (exact: e4m3 is a subset of f16), bf16 queries too, each row scaled by a power
 //     of two.  K's scale multiplies the scores, V's scale the product of its keys: no operand is rounded again but
 //     P, to f16.
@@ -28,15 +28,15 @@
 namespace kcg {
 
 int* device_status_word();
+int encode_tmap(CUtensorMap* out, int dtype, const void* base, int rank, const uint64_t* dims,
+                const uint64_t* strides_bytes, const uint32_t* box, int swizzle_bytes);
 
 namespace {
-using sm100::smem_u32;
+using namespace sm100;
 
-constexpr int ROWS = 16;            // query rows of an item
 constexpr int WARPS = 4;
 constexpr int WKEYS = 32;           // keys of a warp's tile
 constexpr int UNIT = WARPS * WKEYS; // keys of a unit
-constexpr int STAGES = 3;
 constexpr float kLazy = 8.0f;       // rescale only when the maximum grew by more than 2^8 (p <= 2^8 fits f16)
 
 struct CachedParams {
@@ -44,10 +44,6 @@ struct CachedParams {
   int64_t q_st, q_sh;
   void* O;
   int64_t o_st, o_sh;
-  const uint8_t* kc;
-  int64_t kc_p, kc_h, kc_t;
-  const uint8_t* vc;
-  int64_t vc_p, vc_h, vc_t;
   const float* ks;
   const float* vs;
   const int32_t* table;
@@ -56,9 +52,10 @@ struct CachedParams {
   const int32_t* cu;                // NULL: `uniform` queries each
   int64_t T, uniform, num_pages;
   int B, Hkv, G, page, causal;
+  int box;                          // rows of a TMA box: 32 where a page is a multiple of that, else 16
   float scale_log2;
-  float* part_o;                    // [grid][2][D/8 * 4][32 lanes]
-  float* part_ml;                   // [grid][2][ROWS][2]
+  float* part_o;                    // [grid][2][NQ D / 4][32 lanes]
+  float* part_ml;                   // [grid][2][8 NQ][2]
   int* meta;                        // [grid][8]
   int* status;
 };
@@ -88,22 +85,20 @@ __device__ __forceinline__ Request request_of(const CachedParams& p, int i) {
   return r;
 }
 __device__ __forceinline__ int unit_tiles(int len) { return len > 0 ? (len + UNIT - 1) / UNIT : 1; }
-__device__ __forceinline__ int row_blocks(const CachedParams& p, int n) {
-  return static_cast<int>((static_cast<int64_t>(n) * p.G + ROWS - 1) / ROWS);
-}
-__device__ __forceinline__ int64_t request_units(const CachedParams& p, const Request& r) {
-  return static_cast<int64_t>(p.Hkv) * row_blocks(p, r.n) * unit_tiles(r.len);
+template <int ROWS> __device__ __forceinline__ int row_blocks(const CachedParams& p, int n) { return (n * p.G + ROWS - 1) / ROWS; }
+template <int ROWS> __device__ __forceinline__ int64_t request_units(const CachedParams& p, const Request& r) {
+  return static_cast<int64_t>(p.Hkv) * row_blocks<ROWS>(p, r.n) * unit_tiles(r.len);
 }
 
 // A place in the batch's sequence of units.
-struct Cursor {
+template <int ROWS> struct Cursor {
   Request r;
   int i, h, rb, tile, tiles, nrb;
   __device__ __forceinline__ void enter(const CachedParams& p, int req, int64_t offset) {
     i = req;
     r = request_of(p, i);
     tiles = unit_tiles(r.len);
-    nrb = row_blocks(p, r.n);
+    nrb = row_blocks<ROWS>(p, r.n);
     const int64_t item = offset / tiles;
     tile = static_cast<int>(offset - item * tiles);
     h = static_cast<int>(item / nrb);
@@ -122,19 +117,12 @@ struct Cursor {
           r = request_of(p, i);
         } while (r.n == 0);
         tiles = unit_tiles(r.len);
-        nrb = row_blocks(p, r.n);
+        nrb = row_blocks<ROWS>(p, r.n);
       }
     }
     return true;
   }
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
-  const int bytes = take ? 16 : 0;   // 0: sixteen zero bytes, the source is not read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
@@ -151,68 +139,83 @@ __device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t& lo, uint32_t
       : "r"(w));
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {   // c = a b
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// 8x8 16-bit transpose across the warp: lane (g, t) gives row g, columns 2t and 2t + 1, and gets column g, rows 2t, 2t + 1
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// over the eight lanes that share t = lane % 4
+__device__ __forceinline__ float column_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xffffffffu, v, 1);
-  return v + __shfl_xor_sync(0xffffffffu, v, 2);
+__device__ __forceinline__ float column_sum(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
-// Byte offset of 16-byte chunk c of row r inside a tile of D-byte rows: chunks are permuted inside 128-byte lines so
-// that both readings are free of bank conflicts: K by (row = lane / 4, chunk = lane % 4 (+ 4)), V by
-// (row = 2 (lane % 4) + const, chunk = lane / 4).
+// Byte offset of 16-byte chunk c of row r inside a tile of D-byte rows: TMA's swizzle of D bytes (the chunk's number
+// xor that of its 128-byte line).  K is read by (row = lane / 4, chunk = lane % 4 (x 2 + c)), V by (row = 2 (lane % 4) + const, chunk = lane / 4):
+// at D = 128 both are free of bank conflicts, at D = 64 V's 8-byte reads meet in pairs.
 template <int D> __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
-  if constexpr (D == 128) {
-    return r * 128 + ((c ^ ((((r >> 1) & 3) << 1) ^ ((r & 1) << 2))) << 4);
-  } else {
-    const int line = r >> 1;
-    return line * 128 + (((((r & 1) << 2) | c) ^ ((line & 3) << 1)) << 4);
-  }
+  if constexpr (D == 128) return r * 128 + ((c ^ (r & 7)) << 4);
+  else return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
 }
 
-template <int D> struct SplitSmem {
+// Blocks per SM and ring stages: what the registers of 8 NQ rows leave room for.
+template <int NQ> struct SplitShape { static constexpr int BLOCKS = NQ == 1 ? 3 : 2, STAGES = NQ == 1 ? 2 : 3; };
+
+template <int D, int NQ> struct SplitSmem {
+  static constexpr int STAGES = SplitShape<NQ>::STAGES;
   static constexpr int TILE = WKEYS * D;              // bytes of a K or V tile of one warp
-  static constexpr int NREG = D / 2;                  // output registers of a lane
+  static constexpr int NREG = NQ * D / 4;             // output registers of a lane
   uint8_t ring[WARPS][STAGES][2][TILE];
-  float fold[2][NREG][32];                            // a warp's output on its way into another's
-  float fold_ml[2][ROWS][2];
-  float side[WARPS][STAGES][8];                       // per half tile: k scale, v scale, keys
+  static constexpr int FOLDS = NQ == 1 ? 2 : 1;       // (two do not fit beside a ring of three stages)
+  float fold[FOLDS][NREG][32];                        // a warp's output on its way into another's
+  float fold_ml[FOLDS][8 * NQ][2];
+  float side[WARPS][STAGES][8];                       // per half tile: k scale (2), v scale (2), keys (2)
+  uint64_t full[WARPS][STAGES];
   int64_t scan[WARPS];
-  int64_t total;
   int64_t start_off;
   int start_i;
+  int abort;
 };
 
-// Query fragments of an item: lane (g, t) holds rows g and g + 8, for every 16-wide step of the products four
-// dims of each (the dims of step s are those lane t's K words of step s hold).  Scaled to f16's range by a power of
-// two per row; `f` receives its inverse.
-template <typename T, int D>
-__device__ __forceinline__ void load_queries(const CachedParams& p, const Cursor& c, int lane, uint32_t (&qa)[D / 16][4], float (&f)[2]) {
+// Query fragments of an item: lane (g, t) holds row 8 q + g of tile q, for every 16-wide step s of the product the four
+// dims that lane t's K words of that step hold, (D / 4) t + 4 s and on.  bf16 rows are scaled to f16's range by a power of two; f[q] receives
+// its inverse for rows 8 q + 2 t and 8 q + 2 t + 1, the columns of S^T this lane will hold.
+template <typename T, int D, int NQ>
+__device__ __forceinline__ void load_queries(const CachedParams& p, const Cursor<8 * NQ>& c, int lane, uint32_t (&qb)[NQ][D / 16][2],
+                                             float (&f)[NQ][2]) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int R = c.rb * ROWS + g + 8 * half;
+  for (int q = 0; q < NQ; ++q) {
+    const int R = c.rb * (8 * NQ) + 8 * q + g;
     uint4 v[D / 32];
     const bool live = R < c.r.n * p.G;
     const int j = live ? R / p.G : 0;
-    const T* q = static_cast<const T*>(p.Q) + (c.r.t0 + j) * p.q_st + (c.h * p.G + (live ? R - j * p.G : 0)) * p.q_sh;
+    const T* src = static_cast<const T*>(p.Q) + (c.r.t0 + j) * p.q_st + (c.h * p.G + (live ? R - j * p.G : 0)) * p.q_sh;
 #pragma unroll
-    for (int k = 0; k < D / 64; ++k)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        v[2 * k + e] = live ? __ldg(reinterpret_cast<const uint4*>(q + 64 * k + 16 * t) + e) : make_uint4(0, 0, 0, 0);
-    f[half] = 1.f;
-    if constexpr (sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value) {
+    for (int k = 0; k < D / 32; ++k)
+      v[k] = live ? __ldg(reinterpret_cast<const uint4*>(src + (D / 4) * t) + k) : make_uint4(0, 0, 0, 0);
+    f[q][0] = f[q][1] = 1.f;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
       uint32_t m = 0;
 #pragma unroll
       for (int k = 0; k < D / 32; ++k) {
@@ -227,7 +230,9 @@ __device__ __forceinline__ void load_queries(const CachedParams& p, const Cursor
       int e = static_cast<int>(m >> 7) - 127 - 13;
       e = e < -113 ? -113 : e;
       const float up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      f[half] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      const float down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      f[q][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+      f[q][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
 #pragma unroll
       for (int k = 0; k < D / 32; ++k) {
         uint32_t* w = reinterpret_cast<uint32_t*>(&v[k]);
@@ -236,63 +241,70 @@ __device__ __forceinline__ void load_queries(const CachedParams& p, const Cursor
       }
     }
 #pragma unroll
-    for (int s = 0; s < D / 16; ++s) {      // step s: word s % 4 of chunk s / 4, i.e. dims 64 (s / 4) + 16 t + 4 (s % 4) ..
-      const uint4 x = v[2 * (s / 4) + ((s % 4) >> 1)];
-      qa[s][half] = (s & 1) ? x.z : x.x;
-      qa[s][2 + half] = (s & 1) ? x.w : x.y;
+    for (int s = 0; s < D / 16; ++s) {
+      const uint4 x = v[s / 2];
+      qb[q][s][0] = (s & 1) ? x.z : x.x;
+      qb[q][s][1] = (s & 1) ? x.w : x.y;
     }
   }
 }
 
-// Output tiles [j0, j0 + N) of an item, divided by the row sums.  Lane (g, t) holds of tile j rows g (registers 0, 1)
-// and g + 8 (2, 3), dims 2 t (D / 8) + j and (2 t + 1) (D / 8) + j.
+// A lane's share of an item's output, divided by the row sums.  Lane (g, t) holds of tile q rows 8 q + 2 t + e (e = 0, 1),
+// dims (D / 8) g + 2 j + half in o[j][2 half + e]; here tiles j0 .. j0 + N - 1.
 template <typename T, int D, int N>
-__device__ __forceinline__ void store_rows(const CachedParams& p, int t0, int n, int h, int rb, int lane, const float (&o)[N][4],
+__device__ __forceinline__ void store_rows(const CachedParams& p, int t0, int n, int h, int row, int lane, const float (&o)[N][4],
                                            const float (&l)[2], int j0) {
   const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int R = rb * ROWS + g + 8 * half;
+  for (int e = 0; e < 2; ++e) {
+    const int R = row + 2 * t + e;
     if (R >= n * p.G) continue;
     const int j = R / p.G;
-    T* dst = static_cast<T*>(p.O) + (t0 + j) * p.o_st + (h * p.G + (R - j * p.G)) * p.o_sh + 2 * t * (D / 8) + j0;
-    const float inv = l[half] == 0.f ? 0.f : 1.0f / l[half];    // a row that sees no key is zero
+    T* dst = static_cast<T*>(p.O) + (t0 + j) * p.o_st + (h * p.G + (R - j * p.G)) * p.o_sh + g * (D / 8) + 2 * j0;
+    const float inv = l[e] == 0.f ? 0.f : 1.0f / l[e];    // a row that sees no key is zero
+    uint32_t w[N];
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      if constexpr (N % 8 == 0) {
+    for (int k = 0; k < N; ++k) {
+      const float v[2] = {o[k][e] * inv, o[k][2 + e] * inv};
+      w[k] = Words<T>::pack(v);
+    }
+    if constexpr (N % 4 == 0) {
 #pragma unroll
-        for (int k = 0; k < N; k += 8) {
-          uint32_t w[4];
+      for (int k = 0; k < N; k += 4) reinterpret_cast<uint4*>(dst)[k / 4] = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+    } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float v[2] = {o[k + 2 * e][2 * half + side] * inv, o[k + 2 * e + 1][2 * half + side] * inv};
-            w[e] = Words<T>::pack(v);
-          }
-          *reinterpret_cast<uint4*>(dst + side * (D / 8) + k) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) dst[side * (D / 8) + k] = Conv<T>::from_f(o[k][2 * half + side] * inv);
-      }
+      for (int k = 0; k < N; ++k) reinterpret_cast<uint32_t*>(dst)[k] = w[k];
     }
   }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(WARPS * 32, 2) cached_split_kernel(const CachedParams p) {
-  extern __shared__ __align__(128) uint8_t smem_raw[];
-  SplitSmem<D>& sm = *reinterpret_cast<SplitSmem<D>*>(smem_raw);
-  constexpr int NT = D / 8;                 // output tiles of 8 dims
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(WARPS * 32, SplitShape<NQ>::BLOCKS)
+cached_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const CachedParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  using Smem = SplitSmem<D, NQ>;
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  constexpr int ROWS = 8 * NQ, STAGES = Smem::STAGES, NREG = Smem::NREG;
+  constexpr int MT = D / 16;                // output tiles of 16 dims
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   grid_launch_dependents();
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) mbar_init(&sm.full[warp][s], 1);
+    if (warp == 0) {
+      prefetch_tmap(&tmK);
+      prefetch_tmap(&tmV);
+      sm.abort = 0;
+    }
+    mbar_fence_init();
+  }
   grid_dependency_wait();
 
   // ---- this block's range of units ----
   const int per = (p.B + WARPS * 32 - 1) / (WARPS * 32);
   const int i_lo = min(tid * per, p.B), i_hi = min(i_lo + per, p.B);
   int64_t mine = 0;
-  for (int i = i_lo; i < i_hi; ++i) mine += request_units(p, request_of(p, i));
+  for (int i = i_lo; i < i_hi; ++i) mine += request_units<ROWS>(p, request_of(p, i));
   int64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -315,7 +327,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) cached_split_kernel(const Cache
     int64_t off = u0 - (upto - mine);
     int i = i_lo;
     for (;; ++i) {
-      const int64_t n = request_units(p, request_of(p, i));
+      const int64_t n = request_units<ROWS>(p, request_of(p, i));
       if (off < n) break;
       off -= n;
     }
@@ -324,175 +336,194 @@ __global__ void __launch_bounds__(WARPS * 32, 2) cached_split_kernel(const Cache
   }
   __syncthreads();
 
-  Cursor cur;
+  Cursor<ROWS> cur;
   cur.enter(p, sm.start_i, sm.start_off);
   const int units = static_cast<int>(u1 - u0);
 
   // ---- loading: a cursor of its own, running ahead ----
-  Cursor ld = cur;
+  Cursor<ROWS> ld = cur;
   int ld_unit = 0;
-  int pid = -1, pid_tile = -1 << 20;        // this lane's page (tile pid_tile + lane / 2, half lane & 1), and its scales
+  // this lane's look-ahead: page, row in it and scales of half lane & 1 of tile pid_tile + lane / 2
+  int pid = -1, pid_row = 0, pid_tile = -1 << 20;
   float pid_ks = 0.f, pid_vs = 0.f;
   auto load_next = [&](int stage) {
-    if (ld_unit < units) {
-      if (ld.tile < pid_tile || ld.tile >= pid_tile + 16) {
-        pid_tile = ld.tile;
-        const int key = (ld.tile + (lane >> 1)) * UNIT + warp * WKEYS + (lane & 1) * 16;
-        pid = -1;
-        if (key < ld.r.len) {
-          pid = p.table[ld.i * p.table_stride + key / p.page];
-          if (pid < 0 || pid >= p.num_pages) {
-            pid = -1;
-            if (p.status) *p.status = KCG_ERR_INVALID_ARG;
-          }
-        }
-        pid_ks = pid_vs = 0.f;
-        if (pid >= 0) {
-          pid_ks = p.ks[static_cast<int64_t>(pid) * p.Hkv + ld.h];
-          pid_vs = p.vs[static_cast<int64_t>(pid) * p.Hkv + ld.h];
+    if (ld_unit >= units) return;
+    if (ld.tile < pid_tile || ld.tile >= pid_tile + 16) {
+      pid_tile = ld.tile;
+      const int key = (ld.tile + (lane >> 1)) * UNIT + warp * WKEYS + (lane & 1) * 16;
+      pid = -1;
+      pid_row = 0;
+      if (key < ld.r.len) {
+        const int w = key / p.page;
+        pid_row = key - w * p.page;
+        pid = p.table[ld.i * p.table_stride + w];
+        if (pid < 0 || pid >= p.num_pages) {
+          pid = -1;
+          if (p.status) *p.status = KCG_ERR_INVALID_ARG;
         }
       }
-      const int at = ld.tile - pid_tile;
-      const int key0 = ld.tile * UNIT + warp * WKEYS;
-      if ((lane >> 1) == at) {
-        float* s = sm.side[warp][stage] + (lane & 1);
-        s[0] = pid_ks;
-        s[2] = pid_vs;
-        reinterpret_cast<int*>(s)[4] = pid >= 0 ? min(16, ld.r.len - (key0 + (lane & 1) * 16)) : 0;
-      }
-      const uint32_t kdst = smem_u32(sm.ring[warp][stage][0]), vdst = smem_u32(sm.ring[warp][stage][1]);
-      constexpr int CPR = D / 16;           // chunks of a row
-      constexpr int RPI = 32 / CPR;         // rows of one warp instruction
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int64_t pg = __shfl_sync(0xffffffffu, pid, 2 * at + half);
-        const int key = key0 + half * 16;
-        const int in = key % p.page;
-        const uint8_t* ksrc = p.kc + (pg < 0 ? 0 : pg) * p.kc_p + ld.h * p.kc_h + (lane % CPR) * 16;
-        const uint8_t* vsrc = p.vc + (pg < 0 ? 0 : pg) * p.vc_p + ld.h * p.vc_h + (lane % CPR) * 16;
-        const int have = pg < 0 ? 0 : ld.r.len - key;
-#pragma unroll
-        for (int q = 0; q < 16 / RPI; ++q) {
-          const int r = q * RPI + lane / CPR;
-          const bool take = r < have;
-          const int64_t row = take ? in + r : 0;
-          const uint32_t at_s = tile_offset<D>(half * 16 + r, lane % CPR);
-          cp_async16(kdst + at_s, ksrc + row * p.kc_t, take);
-          cp_async16(vdst + at_s, vsrc + row * p.vc_t, take);
-        }
-      }
-      if (++ld_unit < units) {
-        if (ld.next(p)) pid_tile = -1 << 20;
+      pid_ks = pid_vs = 0.f;
+      if (pid >= 0) {
+        pid_ks = p.ks[static_cast<int64_t>(pid) * p.Hkv + ld.h];
+        pid_vs = p.vs[static_cast<int64_t>(pid) * p.Hkv + ld.h];
       }
     }
-    cp_async_commit();
+    const int at = ld.tile - pid_tile;
+    if ((lane >> 1) == at) {
+      float* s = sm.side[warp][stage] + (lane & 1);
+      s[0] = pid_ks;
+      s[2] = pid_vs;
+      reinterpret_cast<int*>(s)[4] = pid >= 0 ? min(16, ld.r.len - (ld.tile * UNIT + warp * WKEYS + (lane & 1) * 16)) : 0;
+    }
+    const int pg0 = __shfl_sync(0xffffffffu, pid, 2 * at), pg1 = __shfl_sync(0xffffffffu, pid, 2 * at + 1);
+    const int in0 = __shfl_sync(0xffffffffu, pid_row, 2 * at), in1 = __shfl_sync(0xffffffffu, pid_row, 2 * at + 1);
+    if (lane == 0) {
+      // rows behind the last token are loaded with their page and left out by the reader; a half tile of no page is not
+      // loaded at all (with boxes of 32 rows both halves are one page's, and the second may only lie behind the end)
+      uint8_t* kdst = sm.ring[warp][stage][0];
+      uint8_t* vdst = sm.ring[warp][stage][1];
+      uint64_t* bar = &sm.full[warp][stage];
+      const bool second = pg1 >= 0 && p.box == 16;
+      mbar_expect_tx(bar, 2 * D * ((pg0 >= 0 ? p.box : 0) + (second ? 16 : 0)));
+      if (pg0 >= 0) {
+        tma_load_4d(kdst, &tmK, bar, 0, in0, ld.h, pg0);
+        tma_load_4d(vdst, &tmV, bar, 0, in0, ld.h, pg0);
+      }
+      if (second) {
+        tma_load_4d(kdst + 16 * D, &tmK, bar, 0, in1, ld.h, pg1);
+        tma_load_4d(vdst + 16 * D, &tmV, bar, 0, in1, ld.h, pg1);
+      }
+    }
+    if (++ld_unit < units) {
+      if (ld.next(p)) pid_tile = -1 << 20;
+    }
   };
+  __syncwarp();
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) load_next(s);
 
-  uint32_t qa[D / 16][4];
-  float qf[2];
-  float o[NT][4], m[2], l[2];
+  uint32_t qb[NQ][D / 16][2];
+  float cq[NQ][2];                          // what a score of this lane's columns is multiplied with, but for K's scale
+  float o[NQ][MT][4], m[NQ][2], l[NQ][2];
   bool fresh = true;
   int stage = 0;
   bool first_item = true;
   int item_tile0 = cur.tile;                // of the part of the item this block has
+  int lim0 = 0;                             // first key the item's first row must not see
+  uint32_t parity = 0;
   for (int u = 0; u < units; ++u) {
-    cp_async_wait<STAGES - 2>();
-    __syncwarp();
+    __syncwarp();                           // every lane has read the tile that is replaced now
     load_next(stage == 0 ? STAGES - 1 : stage - 1);
     if (fresh) {
-      load_queries<T, D>(p, cur, lane, qa, qf);
+      load_queries<T, D, NQ>(p, cur, lane, qb, cq);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
+      for (int q = 0; q < NQ; ++q) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j) o[q][j][0] = o[q][j][1] = o[q][j][2] = o[q][j][3] = 0.f;
+        m[q][0] = m[q][1] = -INFINITY;
+        l[q][0] = l[q][1] = 0.f;
+        cq[q][0] *= p.scale_log2;
+        cq[q][1] *= p.scale_log2;
+      }
       fresh = false;
       item_tile0 = cur.tile;
+      lim0 = p.causal ? cur.r.len - cur.r.n + 1 + cur.rb * ROWS / p.G : INT32_MAX;
     }
+    // A wait that runs out of time marks the launch as failed and goes on with what is there: the barriers that follow
+    // need every warp, and the status tells the host that the result is void.
+    if (!mbar_wait(&sm.full[warp][stage], parity, &sm.abort) && !*static_cast<volatile int*>(&sm.abort)) {
+      *static_cast<volatile int*>(&sm.abort) = 1;
+      if (p.status) *p.status = KCG_ERR_TIMEOUT;
+    }
+    __syncwarp();
     const uint32_t kt = smem_u32(sm.ring[warp][stage][0]), vt = smem_u32(sm.ring[warp][stage][1]);
     const float* side = sm.side[warp][stage];
     const int key0 = cur.tile * UNIT + warp * WKEYS;
     const int have0 = reinterpret_cast<const int*>(side)[4], have1 = reinterpret_cast<const int*>(side)[5];
-    // ---- scores ----
-    float s[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t w[4];
-        lds128(kt + tile_offset<D>(8 * j + g, t + 4 * c), w);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          uint32_t b0, b1;
-          e4m3x4_to_f16(w[x], b0, b1);
-          mma16816(s[j], qa[4 * c + x], b0, b1);
-        }
-      }
-    }
-    const float c0 = p.scale_log2 * qf[0], c1 = p.scale_log2 * qf[1];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float ks = side[j >> 1];
-      const float f0 = c0 * ks, f1 = c1 * ks;
-      s[j][0] *= f0;
-      s[j][1] *= f0;
-      s[j][2] *= f1;
-      s[j][3] *= f1;
-    }
-    // ---- mask: keys this row must not see, keys that are not there ----
     const int R0 = cur.rb * ROWS;
-    const int past = cur.r.len - cur.r.n + 1;
-    if (have0 < 16 || have1 < 16 || (p.causal && key0 + WKEYS > past + R0 / p.G)) {
-      int lim[2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-        lim[half] = p.causal ? past + (R0 + g + 8 * half) / p.G : cur.r.len;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int k = 8 * j + 2 * t + (e & 1);
-          if ((k & 15) >= (j < 2 ? have0 : have1) || key0 + k >= lim[e >> 1]) s[j][e] = -INFINITY;
-        }
-    }
-    // ---- running maximum ----
-    float grow[2];
+    if ((have0 | have1) > 0) {
+    // ---- scores, S^T: element x of half u is key 16 u + g + 8 (x / 2), row 2 t + (x & 1) of its tile ----
+    float s[NQ][2][4];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      float x = fmaxf(fmaxf(s[0][2 * half], s[0][2 * half + 1]), fmaxf(s[1][2 * half], s[1][2 * half + 1]));
-      x = fmaxf(x, fmaxf(fmaxf(s[2][2 * half], s[2][2 * half + 1]), fmaxf(s[3][2 * half], s[3][2 * half + 1])));
-      x = quad_max(x);
-      grow[half] = 1.f;
-      if (x > m[half] + kLazy || (m[half] == -INFINITY && x > -INFINITY)) {
-        grow[half] = exp2f_approx(m[half] - x);      // 0 for the first keys
-        m[half] = x;
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t w0[4], w1[4];
+        lds128(kt + tile_offset<D>(16 * half + g, (D / 64) * t + c), w0);
+        lds128(kt + tile_offset<D>(16 * half + 8 + g, (D / 64) * t + c), w1);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t a[4];
+          e4m3x4_to_f16(w0[x], a[0], a[2]);
+          e4m3x4_to_f16(w1[x], a[1], a[3]);
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            if (c == 0 && x == 0) mma16816_first(s[q][half], a, qb[q][0][0], qb[q][0][1]);
+            else mma16816(s[q][half], a, qb[q][4 * c + x][0], qb[q][4 * c + x][1]);
+          }
+        }
+      }
+      const float ks = side[half];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s[q][half][x] *= cq[q][x & 1] * ks;
+    }
+    // ---- mask: keys a row must not see, keys that are not there ----
+    const bool ragged = have0 < 16 || have1 < 16;
+    if (ragged || key0 + WKEYS > lim0) {
+      const int past = cur.r.len - cur.r.n + 1;
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int lim = p.causal ? past + (R0 + 8 * q + 2 * t + e) / p.G : cur.r.len;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int in = g + 8 * (k & 1);
+            if (in >= (k < 2 ? have0 : have1) || key0 + 16 * (k >> 1) + in >= lim) s[q][k >> 1][2 * (k & 1) + e] = -INFINITY;
+          }
+        }
+    }
+    // ---- running maximum: changed only when some row outgrows it by 2^kLazy (or has its first keys) ----
+    bool outgrown = false;
+    float top[NQ][2];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        top[q][e] = fmaxf(fmaxf(s[q][0][e], s[q][0][2 + e]), fmaxf(s[q][1][e], s[q][1][2 + e]));
+        outgrown = outgrown || top[q][e] > m[q][e] + kLazy;
+      }
+    if (__any_sync(0xffffffffu, outgrown)) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float x = fmaxf(m[q][e], column_max(top[q][e]));
+          const float grow = x == m[q][e] ? 1.f : exp2f_approx(m[q][e] - x);      // 0 for the first keys
+          m[q][e] = x;
+          l[q][e] *= grow;
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            o[q][j][e] *= grow;
+            o[q][j][2 + e] *= grow;
+          }
+        }
+    }
+    uint32_t pb[NQ][2][2];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const float b0 = m[q][0] == -INFINITY ? 0.f : m[q][0], b1 = m[q][1] == -INFINITY ? 0.f : m[q][1];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float p0 = exp2f_approx(s[q][k >> 1][2 * (k & 1)] - b0), p1 = exp2f_approx(s[q][k >> 1][2 * (k & 1) + 1] - b1);
+        l[q][0] += p0;
+        l[q][1] += p1;
+        pb[q][k >> 1][k & 1] = transpose8x8(pack_f16(p0, p1));
       }
     }
-    if (__any_sync(0xffffffffu, grow[0] != 1.f || grow[1] != 1.f)) {
-      l[0] *= grow[0];
-      l[1] *= grow[1];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        o[j][0] *= grow[0];
-        o[j][1] *= grow[0];
-        o[j][2] *= grow[1];
-        o[j][3] *= grow[1];
-      }
-    }
-    const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
-    uint32_t pa[2][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float p0 = exp2f_approx(s[j][0] - b0), p1 = exp2f_approx(s[j][1] - b0);
-      const float p2 = exp2f_approx(s[j][2] - b1), p3 = exp2f_approx(s[j][3] - b1);
-      l[0] += p0 + p1;
-      l[1] += p2 + p3;
-      pa[j >> 1][(j & 1) * 2] = pack_f16(p0, p1);
-      pa[j >> 1][(j & 1) * 2 + 1] = pack_f16(p2, p3);
-    }
-    // ---- output: the product of each half with its page's scale ----
+    // ---- output, O^T: the product of each half tile with its page's scale ----
     const float vs0 = side[2], vs1 = side[3];
     const bool same = vs0 == vs1;
     constexpr int VW = D / 32;              // words of a lane's share of a V row
@@ -504,107 +535,135 @@ __global__ void __launch_bounds__(WARPS * 32, 2) cached_split_kernel(const Cache
         const int row = half * 16 + 2 * t + (k & 1) + 8 * (k >> 1);
         if constexpr (D == 128) lds128(vt + tile_offset<D>(row, g), v[half][k]);
         else lds64(vt + tile_offset<D>(row, g >> 1) + (g & 1) * 8, v[half][k]);
-      }
-    auto product = [&](int half, int c, float (&acc)[4][4]) {   // += P_half V_half for output tiles 4 c .. 4 c + 3
-      uint32_t b[4][2];
+        // what lies behind the last token may be anything: P is zero there, and so must V be
+        if (ragged && row - half * 16 >= (half ? have1 : have0))
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t x = v[half][2 * k][c], y = v[half][2 * k + 1][c];
-        e4m3x4_to_f16(__byte_perm(x, y, 0x5140), b[0][k], b[1][k]);
-        e4m3x4_to_f16(__byte_perm(x, y, 0x7362), b[2][k], b[3][k]);
+          for (int c = 0; c < VW; ++c) v[half][k][c] = 0;
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mma16816(acc[e], pa[half], b[e][0], b[e][1]);
-    };
+    for (int c = 0; c < VW; ++c) {          // word c: output tiles 2 c and 2 c + 1
+      uint32_t a[2][2][4];
 #pragma unroll
-    for (int c = 0; c < VW; ++c) {
-      float acc[4][4];
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e][0] = acc[e][1] = acc[e][2] = acc[e][3] = 0.f;
-      product(0, c, acc);
-      if (!same) {
+        for (int k = 0; k < 2; ++k) {       // keys 2 t, 2 t + 1, then those + 8
+          const uint32_t x = v[half][2 * k][c], y = v[half][2 * k + 1][c];
+          e4m3x4_to_f16(__byte_perm(x, y, 0x5140), a[half][0][2 * k], a[half][0][2 * k + 1]);
+          e4m3x4_to_f16(__byte_perm(x, y, 0x7362), a[half][1][2 * k], a[half][1][2 * k + 1]);
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+      for (int q = 0; q < NQ; ++q)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            o[4 * c + e][x] = fmaf(acc[e][x], vs0, o[4 * c + e][x]);
-            acc[e][x] = 0.f;
+        for (int e = 0; e < 2; ++e) {
+          float acc[4];
+          float (&out)[4] = o[q][2 * c + e];
+          mma16816_first(acc, a[0][e], pb[q][0][0], pb[q][0][1]);
+          if (same) {
+            mma16816(acc, a[1][e], pb[q][1][0], pb[q][1][1]);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) out[x] = fmaf(acc[x], vs0, out[x]);
+            mma16816_first(acc, a[1][e], pb[q][1][0], pb[q][1][1]);
           }
-      }
-      product(1, c, acc);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) o[4 * c + e][x] = fmaf(acc[e][x], vs1, o[4 * c + e][x]);
+          for (int x = 0; x < 4; ++x) out[x] = fmaf(acc[x], vs1, out[x]);
+        }
     }
 
-    if (++stage == STAGES) stage = 0;
+    }
+    if (++stage == STAGES) {
+      stage = 0;
+      parity ^= 1;
+    }
     const bool last = u + 1 == units;
     if (cur.tile + 1 < cur.tiles && !last) {
       ++cur.tile;
       continue;
     }
     // ---- end of the item, or of this block's part of it: the four warps' results into warp 0 ----
-    l[0] = quad_sum(l[0]);
-    l[1] = quad_sum(l[1]);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      l[q][0] = column_sum(l[q][0]);
+      l[q][1] = column_sum(l[q][1]);
+    }
     auto give = [&](int to) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int q = 0; q < NQ; ++q) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) sm.fold[to][4 * j + x][lane] = o[j][x];
-      if (t == 0) {
-        sm.fold_ml[to][g][0] = m[0];
-        sm.fold_ml[to][g][1] = l[0];
-        sm.fold_ml[to][g + 8][0] = m[1];
-        sm.fold_ml[to][g + 8][1] = l[1];
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) sm.fold[to][(q * MT + j) * 4 + x][lane] = o[q][j][x];
+        if (g == 0)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            sm.fold_ml[to][8 * q + 2 * t + e][0] = m[q][e];
+            sm.fold_ml[to][8 * q + 2 * t + e][1] = l[q][e];
+          }
       }
     };
     auto take = [&](int from) {
-      float mine_w[2], other_w[2];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const float m2 = sm.fold_ml[from][g + 8 * half][0], l2 = sm.fold_ml[from][g + 8 * half][1];
-        const float top = fmaxf(m[half], m2), base = top == -INFINITY ? 0.f : top;
-        mine_w[half] = exp2f_approx(m[half] - base);
-        other_w[half] = exp2f_approx(m2 - base);
-        l[half] = l[half] * mine_w[half] + l2 * other_w[half];
-        m[half] = top;
+      for (int q = 0; q < NQ; ++q) {
+        float mine_w[2], other_w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float m2 = sm.fold_ml[from][8 * q + 2 * t + e][0], l2 = sm.fold_ml[from][8 * q + 2 * t + e][1];
+          const float hi = fmaxf(m[q][e], m2), base = hi == -INFINITY ? 0.f : hi;
+          mine_w[e] = exp2f_approx(m[q][e] - base);
+          other_w[e] = exp2f_approx(m2 - base);
+          l[q][e] = l[q][e] * mine_w[e] + l2 * other_w[e];
+          m[q][e] = hi;
+        }
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            o[q][j][x] = o[q][j][x] * mine_w[x & 1] + sm.fold[from][(q * MT + j) * 4 + x][lane] * other_w[x & 1];
       }
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          o[j][x] = o[j][x] * mine_w[x >> 1] + sm.fold[from][4 * j + x][lane] * other_w[x >> 1];
     };
     __syncthreads();                        // the fold buffers are free
-    if (warp >= 2) give(warp - 2);
-    __syncthreads();
-    if (warp < 2) take(warp);
-    __syncthreads();
+    if constexpr (Smem::FOLDS == 2) {
+      if (warp >= 2) give(warp - 2);
+      __syncthreads();
+      if (warp < 2) take(warp);
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int w = 3; w > 1; --w) {
+        if (warp == w) give(0);
+        __syncthreads();
+        if (warp == 0) take(0);
+        __syncthreads();
+      }
+    }
     if (warp == 1) give(0);
     __syncthreads();
     if (warp == 0) {
       take(0);
       const bool whole = item_tile0 == 0 && cur.tile + 1 == cur.tiles;
       if (whole) {
-        store_rows<T, D, NT>(p, cur.r.t0, cur.r.n, cur.h, cur.rb, lane, o, l, 0);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) store_rows<T, D, MT>(p, cur.r.t0, cur.r.n, cur.h, R0 + 8 * q, lane, o[q], l[q], 0);
       } else {
         const int slot = first_item ? 0 : 1;
-        float* po = p.part_o + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * (D / 2 * 32) + lane;
+        float* po = p.part_o + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * (NREG * 32) + lane;
+        float* pm = p.part_ml + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * (ROWS * 2);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int q = 0; q < NQ; ++q) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x) po[(4 * j + x) * 32] = o[j][x];
-        if (t == 0) {
-          float* pm = p.part_ml + (static_cast<int64_t>(blockIdx.x) * 2 + slot) * (ROWS * 2);
-          pm[2 * g] = m[0];
-          pm[2 * g + 1] = l[0];
-          pm[2 * (g + 8)] = m[1];
-          pm[2 * (g + 8) + 1] = l[1];
+          for (int j = 0; j < MT; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) po[((q * MT + j) * 4 + x) * 32] = o[q][j][x];
+          if (g == 0)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              pm[2 * (8 * q + 2 * t + e)] = m[q][e];
+              pm[2 * (8 * q + 2 * t + e) + 1] = l[q][e];
+            }
         }
         if (item_tile0 == 0 && lane == 0) {
-          // the item begins in this block: it lists the parts.  Its units end before u0 + u + tiles - tile; block c
-          // holds unit x when c = floor(((x + 1) grid - 1) / total).
+          // the item begins in this block, which lists the parts.  Its last unit is x_end; block c holds unit x
+          // when c = floor(((x + 1) grid - 1) / total).
           const int64_t x_end = u0 + u + (cur.tiles - 1 - cur.tile);
           meta[1] = static_cast<int>(((x_end + 1) * grid - 1) / total);
           meta[2] = slot;
@@ -620,70 +679,119 @@ __global__ void __launch_bounds__(WARPS * 32, 2) cached_split_kernel(const Cache
     first_item = false;
     if (!last) cur.next(p);
   }
-  cp_async_wait<0>();
+  // every tile that was asked for has been waited for; after a timeout, give the rest a little longer to land
+  if (*static_cast<volatile int*>(&sm.abort)) {
+    int zero = 0;
+    for (int s = 0; s < STAGES; ++s) mbar_wait(&sm.full[warp][s], s < stage ? parity : parity ^ 1, &zero, 2000000ull);
+  }
 }
 
-// Merges the parts of items that several blocks worked on; block c takes the item that begins in block c of the
-// split kernel and ends behind it.  Warps take shares of the output registers; parts are added in order.
+// Merges the parts of items that several blocks worked on; block (c, y) takes share y of the output tiles (16 dims x 8
+// rows) of the item that begins in block c of the split kernel and ends behind it.  Its warps share the tiles, and
+// where there are fewer tiles than warps, the parts of a tile; sums are taken in an order that depends on sizes alone.
 constexpr int JOIN_WARPS = 8;
-template <typename T, int D>
+template <typename T, int D, int NQ>
 __global__ void __launch_bounds__(JOIN_WARPS * 32) cached_join_kernel(const CachedParams p) {
-  constexpr int NT = D / 8, MINE = NT / JOIN_WARPS;   // output tiles of a warp
+  extern __shared__ float join_w[];                   // [parts][ROWS]: weight of each part
+  __shared__ float s_l[8 * NQ];
+  __shared__ float s_acc[JOIN_WARPS][4][32];
+  constexpr int MT = D / 16, ROWS = 8 * NQ, NREG = NQ * MT * 4;
   grid_launch_dependents();
   grid_dependency_wait();
   const int* meta = p.meta + blockIdx.x * 8;
   if (meta[0] < 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2;
-  const int last = meta[1];
-  const float* part_o = p.part_o + lane + static_cast<int64_t>(warp) * MINE * 4 * 32;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float acc[MINE][4];
-#pragma unroll
-  for (int j = 0; j < MINE; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-  // first the maximum over the parts, then one weighted sum
-  for (int c = blockIdx.x; c <= last; ++c) {
-    const float* pm = p.part_ml + (static_cast<int64_t>(c) * 2 + (c == static_cast<int>(blockIdx.x) ? meta[2] : 0)) * (ROWS * 2);
-    m[0] = fmaxf(m[0], pm[2 * g]);
-    m[1] = fmaxf(m[1], pm[2 * (g + 8)]);
+  const int c0 = blockIdx.x, parts = meta[1] - c0 + 1, slot = meta[2];
+  auto part_of = [&](int i) { return static_cast<int64_t>(c0 + i) * 2 + (i ? 0 : slot); };
+  // weights: one warp per row
+  for (int r = warp; r < ROWS; r += JOIN_WARPS) {
+    float m = -INFINITY;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.part_ml[(part_of(i) * ROWS + r) * 2]);
+    m = warp_max(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int i = lane; i < parts; i += 32) {
+      const float2 ml = *reinterpret_cast<const float2*>(&p.part_ml[(part_of(i) * ROWS + r) * 2]);
+      const float w = exp2f_approx(ml.x - base);
+      join_w[i * ROWS + r] = w;
+      l += ml.y * w;
+    }
+    l = warp_sum(l);
+    if (lane == 0) s_l[r] = l;
   }
-  const float b0 = m[0] == -INFINITY ? 0.f : m[0], b1 = m[1] == -INFINITY ? 0.f : m[1];
-#pragma unroll 4
-  for (int c = blockIdx.x; c <= last; ++c) {
-    const int64_t part = static_cast<int64_t>(c) * 2 + (c == static_cast<int>(blockIdx.x) ? meta[2] : 0);
-    const float* pm = p.part_ml + part * (ROWS * 2);
-    const float w0 = exp2f_approx(pm[2 * g] - b0), w1 = exp2f_approx(pm[2 * (g + 8)] - b1);
-    l[0] += pm[2 * g + 1] * w0;
-    l[1] += pm[2 * (g + 8) + 1] * w1;
-    const float* po = part_o + part * (D / 2 * 32);
+  __syncthreads();
+  const int tiles = NQ * MT / gridDim.y;              // of this block
+  const int per_tile = tiles < JOIN_WARPS ? JOIN_WARPS / tiles : 1;   // warps that share a tile's parts
+  const int t = lane & 3;
+  for (int k0 = 0; k0 < tiles; k0 += JOIN_WARPS / per_tile) {
+    const int k = blockIdx.y * tiles + k0 + warp / per_tile, q = k / MT;
+    float acc[1][4] = {{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll 8
+    for (int i = warp % per_tile; i < parts; i += per_tile) {
+      const float* po = p.part_o + part_of(i) * (NREG * 32) + k * 128 + lane;
+      const float w0 = join_w[i * ROWS + 8 * q + 2 * t], w1 = join_w[i * ROWS + 8 * q + 2 * t + 1];
 #pragma unroll
-    for (int j = 0; j < MINE; ++j)
+      for (int x = 0; x < 4; ++x) acc[0][x] = fmaf(po[32 * x], x & 1 ? w1 : w0, acc[0][x]);
+    }
+    if (per_tile > 1) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) acc[j][x] = fmaf(po[(4 * j + x) * 32], x < 2 ? w0 : w1, acc[j][x]);
+      for (int x = 0; x < 4; ++x) s_acc[warp][x][lane] = acc[0][x];
+      __syncthreads();
+      if (warp % per_tile == 0)
+        for (int o = 1; o < per_tile; ++o)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[0][x] += s_acc[warp + o][x][lane];
+    }
+    if (warp % per_tile == 0) {
+      const float l[2] = {s_l[8 * q + 2 * t], s_l[8 * q + 2 * t + 1]};
+      store_rows<T, D, 1>(p, meta[3], meta[4], meta[5], meta[6] * ROWS + 8 * q, lane, acc, l, k % MT);
+    }
   }
-  store_rows<T, D, MINE>(p, meta[3], meta[4], meta[5], meta[6], lane, acc, l, warp * MINE);
 }
 
-int split_grid() { return sm_count() * 2; }
+// Workspace of the split kernel with 8 NQ rows: two parts per block, each the lanes' output registers and (m, l) of
+// every row, and eight ints per block.
+size_t split_workspace(int64_t D, int nq, int grid) {
+  return static_cast<size_t>(grid) * (2 * (nq * D / 4 * 32 * 4) + 2 * (8 * nq * 2 * 4) + 32);
+}
+int split_grid(int nq) { return sm_count() * (nq == 1 ? SplitShape<1>::BLOCKS : SplitShape<2>::BLOCKS); }
 
-template <int D> size_t workspace_of(int grid) {
-  return static_cast<size_t>(grid) * (2 * (D / 2 * 32 * 4) + 2 * (ROWS * 2 * 4) + 32);
+// Tensor map of one cache: [page][head][row][D], boxes of `box` rows.
+int cache_map(CUtensorMap* tm, const void* cache, const int64_t strides[3], int64_t D, const CachedParams& p) {
+  const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(p.page), static_cast<uint64_t>(p.Hkv),
+                            static_cast<uint64_t>(p.num_pages)};
+  // the stride of a dim with one entry is never used, but has to be a valid one
+  const uint64_t st[3] = {static_cast<uint64_t>(strides[2]), static_cast<uint64_t>(p.Hkv > 1 ? strides[1] : D),
+                          static_cast<uint64_t>(p.num_pages > 1 ? strides[0] : D)};
+  const uint32_t box[4] = {static_cast<uint32_t>(D), static_cast<uint32_t>(p.box), 1, 1};
+  return encode_tmap(tm, KCG_F8E4M3, cache, 4, dims, st, box, static_cast<int>(D));   // a row is one swizzle span
+}
+
+template <typename T, int D, int NQ>
+int launch_split(CachedParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV, int64_t items, void* workspace, cudaStream_t stream) {
+  const int grid = split_grid(NQ);
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + static_cast<size_t>(grid) * 2 * (NQ * D / 4 * 32);
+  p.meta = reinterpret_cast<int*>(p.part_ml + static_cast<size_t>(grid) * 2 * (8 * NQ * 2));
+  constexpr int SMEM = sizeof(SplitSmem<D, NQ>) + 1024;
+  static_assert(SMEM <= 228 * 1024 / SplitShape<NQ>::BLOCKS - 1024, "the blocks of an SM do not fit its shared memory");
+  auto kern = cached_split_kernel<T, D, NQ>;
+  KCG_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+  launch_overlapped(kern, dim3(grid), dim3(WARPS * 32), SMEM, stream, tmK, tmV, p);
+  const int rc = check_launch("cached_split_kernel");
+  if (rc) return rc;
+  // Many items: few parts each, one block per item.  Few items: many parts each, whose reading is spread over a
+  // block per output tile.
+  const unsigned share = items * 8 <= grid ? NQ * D / 16 : NQ;
+  launch_overlapped(cached_join_kernel<T, D, NQ>, dim3(grid, share), dim3(JOIN_WARPS * 32), (grid + 1) * 8 * NQ * sizeof(float), stream, p);
+  return check_launch("cached_join_kernel");
 }
 
 template <typename T, int D>
-int launch_split(CachedParams& p, void* workspace, cudaStream_t stream) {
-  const int grid = split_grid();
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + static_cast<size_t>(grid) * 2 * (D / 2 * 32);
-  p.meta = reinterpret_cast<int*>(p.part_ml + static_cast<size_t>(grid) * 2 * (ROWS * 2));
-  constexpr int SMEM = sizeof(SplitSmem<D>);
-  auto kern = cached_split_kernel<T, D>;
-  KCG_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-  launch_overlapped(kern, dim3(grid), dim3(WARPS * 32), SMEM, stream, p);
-  const int rc = check_launch("cached_split_kernel");
-  if (rc) return rc;
-  launch_overlapped(cached_join_kernel<T, D>, dim3(grid), dim3(JOIN_WARPS * 32), 0, stream, p);
-  return check_launch("cached_join_kernel");
+int launch_cached(CachedParams& p, int64_t rows, const CUtensorMap& tmK, const CUtensorMap& tmV, void* workspace, cudaStream_t stream) {
+  const int64_t items = static_cast<int64_t>(p.B) * p.Hkv;
+  if (rows <= 8) return launch_split<T, D, 1>(p, tmK, tmV, items, workspace, stream);
+  return launch_split<T, D, 2>(p, tmK, tmV, items * ((rows + 15) / 16), workspace, stream);
 }
 
 }  // namespace
@@ -694,7 +802,8 @@ extern "C" int kcg_fmha_cached_workspace(int64_t D, size_t* bytes) {
   clear_error();
   if (!bytes) return fail(KCG_ERR_INVALID_ARG, "fmha_cached_workspace: null pointer");
   if (D != 64 && D != 128) return fail(KCG_ERR_UNSUPPORTED, "fmha_cached: head dimension %lld has no kernel (64, 128)", static_cast<long long>(D));
-  *bytes = D == 128 ? workspace_of<128>(split_grid()) : workspace_of<64>(split_grid());
+  const size_t one = split_workspace(D, 1, split_grid(1)), two = split_workspace(D, 2, split_grid(2));
+  *bytes = one > two ? one : two;
   return KCG_OK;
 }
 
@@ -726,6 +835,10 @@ extern "C" int kcg_fmha_cached_fwd(int dtype, int64_t T, int64_t B, int64_t Hq, 
   bool ok = aligned16(Q) && aligned16(O) && aligned16(k_cache) && aligned16(v_cache) && aligned16(workspace);
   for (int i = 0; i < 2; ++i) ok = ok && q_strides[i] % 8 == 0 && o_strides[i] % 8 == 0;
   for (int i = 0; i < 3; ++i) ok = ok && kc_strides[i] % 16 == 0 && vc_strides[i] % 16 == 0;
+  if (num_pages == 0) return fail(KCG_ERR_INVALID_ARG, "fmha_cached: the cache has no pages");
+  if ((Hkv > 1 && (kc_strides[1] <= 0 || vc_strides[1] <= 0)) || (num_pages > 1 && (kc_strides[0] <= 0 || vc_strides[0] <= 0)) ||
+      kc_strides[2] <= 0 || vc_strides[2] <= 0)
+    return fail(KCG_ERR_UNSUPPORTED, "fmha_cached: the strides of the caches must be positive");
   if (!ok) return fail(KCG_ERR_ALIGNMENT, "fmha_cached: rows of Q, O, the caches and the workspace must start on 16-byte boundaries");
   size_t need = 0;
   const int rc = kcg_fmha_cached_workspace(D, &need);
@@ -735,18 +848,23 @@ extern "C" int kcg_fmha_cached_fwd(int dtype, int64_t T, int64_t B, int64_t Hq, 
   CachedParams p{};
   p.Q = Q; p.q_st = q_strides[0]; p.q_sh = q_strides[1];
   p.O = O; p.o_st = o_strides[0]; p.o_sh = o_strides[1];
-  p.kc = static_cast<const uint8_t*>(k_cache); p.kc_p = kc_strides[0]; p.kc_h = kc_strides[1]; p.kc_t = kc_strides[2];
-  p.vc = static_cast<const uint8_t*>(v_cache); p.vc_p = vc_strides[0]; p.vc_h = vc_strides[1]; p.vc_t = vc_strides[2];
   p.ks = k_scale; p.vs = v_scale;
   p.table = block_table; p.table_stride = table_stride; p.width = table_width;
   p.lengths = lengths; p.cu = cu_new;
   p.T = T; p.uniform = cu_new ? 0 : T / B; p.num_pages = num_pages;
   p.B = static_cast<int>(B); p.Hkv = static_cast<int>(Hkv); p.G = static_cast<int>(Hq / Hkv);
   p.page = static_cast<int>(page_size); p.causal = causal != 0;
+  p.box = page_size % 32 == 0 ? 32 : 16;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = device_status_word();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // query rows of a request and key head, which choose the kernel: from max_new, else the mean over the batch
+  CUtensorMap tmK, tmV;
+  int mrc = cache_map(&tmK, k_cache, kc_strides, D, p);
+  if (!mrc) mrc = cache_map(&tmV, v_cache, vc_strides, D, p);
+  if (mrc) return mrc;
+  const int64_t rows = (max_new > 0 ? max_new : (T + B - 1) / B) * p.G;
   if (dtype == KCG_BF16)
-    return D == 128 ? launch_split<__nv_bfloat16, 128>(p, workspace, s) : launch_split<__nv_bfloat16, 64>(p, workspace, s);
-  return D == 128 ? launch_split<__half, 128>(p, workspace, s) : launch_split<__half, 64>(p, workspace, s);
+    return D == 128 ? launch_cached<__nv_bfloat16, 128>(p, rows, tmK, tmV, workspace, s) : launch_cached<__nv_bfloat16, 64>(p, rows, tmK, tmV, workspace, s);
+  return D == 128 ? launch_cached<__half, 128>(p, rows, tmK, tmV, workspace, s) : launch_cached<__half, 64>(p, rows, tmK, tmV, workspace, s);
 }

@@ -35,8 +35,8 @@ EncodeTiledFn encode_fn() {
 
 // Encodes a rank-`rank` tensor map with 128-byte swizzle.  dims/strides are innermost
 // first; strides (bytes) are given for dims 1..rank-1.
-int encode_tmap_sw128(CUtensorMap* out, int dtype, const void* base, int rank, const uint64_t* dims,
-                      const uint64_t* strides_bytes, const uint32_t* box) {
+int encode_tmap(CUtensorMap* out, int dtype, const void* base, int rank, const uint64_t* dims,
+                const uint64_t* strides_bytes, const uint32_t* box, int swizzle_bytes) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(KCG_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   CUtensorMapDataType dt;
@@ -52,13 +52,17 @@ int encode_tmap_sw128(CUtensorMap* out, int dtype, const void* base, int rank, c
   for (int i = 0; i < rank; ++i) { gd[i] = dims[i]; bx[i] = box[i]; es[i] = 1; }
   for (int i = 0; i + 1 < rank; ++i) gs[i] = strides_bytes[i];
   CUresult r = fn(out, dt, static_cast<cuuint32_t>(rank), const_cast<void*>(base), gd, gs, bx, es,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle_bytes == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(KCG_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (rank %d, dims %llu x %llu)",
                 static_cast<int>(r), rank, static_cast<unsigned long long>(dims[0]),
                 static_cast<unsigned long long>(rank > 1 ? dims[1] : 1));
   return KCG_OK;
+}
+int encode_tmap_sw128(CUtensorMap* out, int dtype, const void* base, int rank, const uint64_t* dims,
+                      const uint64_t* strides_bytes, const uint32_t* box) {
+  return encode_tmap(out, dtype, base, rank, dims, strides_bytes, box, 128);
 }
 
 namespace {
