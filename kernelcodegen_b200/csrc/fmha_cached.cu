@@ -1015,12 +1015,15 @@ int launch_split(CachedParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV
   return check_launch("cached_join_kernel");
 }
 
+#include "fmha_cached_tiles_kernel.cuh"
+
 template <typename T, int D>
 int launch_cached(CachedParams& p, int64_t rows, const CUtensorMap& tmK, const CUtensorMap& tmV, void* workspace, cudaStream_t stream) {
   const int64_t items = static_cast<int64_t>(p.B) * p.Hkv;
   // Two heads side by side where there are two: as fast as four or one with a head's page in one piece, and 20 % faster
   // than one where a token's heads stand together (8 x 4096 tokens of 32 heads, token-major: 54.8 us, one head 68.2).
   p.wk_log2 = p.Hkv % 2 == 0 ? 1 : 2;
+  if (rows > 16) return launch_tiles<T, D>(p, tmK, tmV, stream);
   if (rows <= 8) return launch_split<T, D, 1>(p, tmK, tmV, items, workspace, stream);
   return launch_split<T, D, 2>(p, tmK, tmV, items * ((rows + 15) / 16), workspace, stream);
 }

@@ -68,7 +68,7 @@ def append(x, slots, code, scale, page):
                 code[p, h, r] = round_e4m3(y)
 
 
-def attend(Q, code, kscale, vcode, vscale, table, lengths, cu, page, scale, causal):
+def attend(Q, code, kscale, vcode, vscale, table, lengths, cu, page, scale, causal, many=False):
     """(O, allowed error) in float64 for Q [T, Hq, D]; rows outside cu are NaN.
 
     What a kernel with fp32 sums and P rounded to fp16 may be off by, with A = sum p |v| / sum p (per element):
@@ -78,6 +78,9 @@ def attend(Q, code, kscale, vcode, vscale, table, lengths, cu, page, scale, caus
       exp2 (2^-22) and the fp32 sums over keys (sequential at worst per lane:
       keys / 8 terms, and the merges)                                         -> (2^-21 + 2 keys/8 2^-24) A,
       the result's own rounding                                               -> eps / 2 |o|.
+    `many`, the kernel for many rows, widens codes to f16 times a power of two, relative to the largest scale: half of
+    f16's smallest step, 2^-25, times that scale per element of K (a score: 2^-25 kmax scale sum |q|, added to d)
+    and V (2^-25 vmax); and it rounds V times what its scale is beside a power of two to f16 -> 2^-11 A.
     """
     T, Hq, D = Q.shape
     Hkv = code.shape[1]
@@ -110,7 +113,11 @@ def attend(Q, code, kscale, vcode, vscale, table, lengths, cu, page, scale, caus
             A = torch.where(l > 0, (p @ V.abs()) / l.clamp_min(1e-300), torch.zeros(()).double())
             rest = torch.where(l > 0, ((p > 0).double() @ V.abs()) / l.clamp_min(1e-300), torch.zeros(()).double())
             d = (D + 8) * 2.0 ** -24 * torch.where(p > 0, size, 0).amax(dim=2, keepdim=True)
-            err = (2.0 ** -11 + 2 * d + 2.0 ** -21 + 2 * (L / 8) * 2.0 ** -24) * A + 2.0 ** -25 * rest
+            small = 0.0
+            if many:
+                d = d + 2.0 ** -25 * float(kscale[ids, h].max()) * abs(scale) * q.abs().sum(dim=2, keepdim=True)
+                small = 2.0 ** -11 * A + 2.0 ** -25 * float(vscale[ids, h].max())
+            err = small + (2.0 ** -11 + 2 * d + 2.0 ** -21 + 2 * (L / 8) * 2.0 ** -24) * A + 2.0 ** -25 * rest
             out[a:b, h * G:(h + 1) * G] = o
             # subnormal results of a 16-bit type are off by half of their smallest step instead
             tiny = torch.finfo(Q.dtype).smallest_normal * half_step

@@ -260,9 +260,9 @@ def make(lengths, new, page, Hq, Hkv, D, dtype, layout="head", seed=0, spread=1.
                 cu_dev=i32(cu).cuda())
 
 
-def check(c, got, softmax_scale, causal):
+def check(c, got, softmax_scale, causal, many=False):
     want, tol = R.attend(c["Q"], c["code"][0].double(), c["scale"][0].double(), c["code"][1].double(),
-                         c["scale"][1].double(), c["table"], c["lengths"], c["cu"], c["page"], softmax_scale, causal)
+                         c["scale"][1].double(), c["table"], c["lengths"], c["cu"], c["page"], softmax_scale, causal, many)
     got = got.cpu().double()
     off = (got - want).abs()
     assert not torch.isnan(got).any()
@@ -295,7 +295,7 @@ def test_attention(case, causal, dtype, layout):
     c = make(lengths, new, page, Hq, Hkv, D, dtype, layout, seed=case)
     got = ops().fmha_cached(*c["args"], c["cu_dev"], softmax_scale=D ** -0.5, causal=causal, max_new=max(new))
     sync_ok()
-    check(c, got, D ** -0.5, causal)
+    check(c, got, D ** -0.5, causal, many=max(new) * Hq // Hkv > 16)
 
 
 @pytest.mark.parametrize("max_new", [0, 1, 7, 10 ** 6])
@@ -303,7 +303,7 @@ def test_attention_max_new_is_only_a_hint(max_new):
     c = make([300, 90, 40], [60, 1, 40], 16, 8, 2, 128, torch.bfloat16, seed=3)
     got = ops().fmha_cached(*c["args"], c["cu_dev"], softmax_scale=0.1, causal=True, max_new=max_new)
     sync_ok()
-    check(c, got, 0.1, True)
+    check(c, got, 0.1, True, many=True)
 
 
 @pytest.mark.parametrize("B,length,new", [(300, 200, 1), (1, 40000, 1), (2000, 20, 1), (3, 9000, 2)])
