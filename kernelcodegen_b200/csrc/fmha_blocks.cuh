@@ -94,8 +94,7 @@ struct NoHook {
 // decided() is called (by all lanes) as soon as this block's value of m is final — before the
 // exponentials on the ordinary path — and wait_o() before the accumulator is touched for a rescale
 // (it returns false if its wait timed out; the rescale is then skipped and the caller gives up).
-// kEmuMask: which pairs of exponentials take the FMA pipe, as KCG_FMHA_EMU_MASK; 0 where a NaN score must stay one.
-template <typename T, int D, int kEmuMask = KCG_FMHA_EMU_MASK, typename Arrive, typename Decided = NoHook, typename WaitO = NoHook>
+template <typename T, int D, typename Arrive, typename Decided = NoHook, typename WaitO = NoHook>
 __device__ __forceinline__ bool softmax_block(uint32_t s_addr, uint32_t o_addr, int j, int limit, float c, float& m,
                                               float& l, int lane, Arrive arrive, Decided decided = Decided(),
                                               WaitO wait_o = WaitO()) {
@@ -128,7 +127,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_addr, uint32_t o_addr, 
     for (int k = half * 64; k < half * 64 + 64; k += 2) {
       const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(sreg[k]), __uint_as_float(sreg[k + 1])), c2, nm2);
       float p0, p1;
-      if (kEmuMask != 0 && ((k >> 1) & kEmuMask) == kEmuMask) {
+      if (KCG_FMHA_EMU_MASK != 0 && ((k >> 1) & KCG_FMHA_EMU_MASK) == KCG_FMHA_EMU_MASK) {
         exp2_pair_fma(x2, p0, p1);
       } else {
         float x0, x1;

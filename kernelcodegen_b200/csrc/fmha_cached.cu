@@ -26,6 +26,7 @@
 #include "common.cuh"
 #include "tcgen05.cuh"
 
+#include <cstddef>
 #include <type_traits>
 
 namespace kcg {
@@ -36,10 +37,11 @@ int encode_tmap(CUtensorMap* out, int dtype, const void* base, int rank, const u
 
 namespace {
 using namespace sm100;
+#include "fmha_blocks.cuh"
 
 constexpr int WARPS = 4;            // of a team
 constexpr int WKEYS = 32;           // keys of a warp's tile
-constexpr float kLazy = 8.0f;       // rescale only when the maximum grew by more than 2^8 (p <= 2^8 fits f16)
+constexpr float kLazy = 14.0f;      // rescale only when the maximum grew by more than 2^14 (p <= 2^14 fits f16)
 
 struct CachedParams {
   const void* Q;
@@ -55,6 +57,7 @@ struct CachedParams {
   int64_t T, uniform, num_pages;
   int B, Hkv, G, page, causal;
   int wk_log2;                      // 2^wk_log2 warps share a head's keys, the others take further heads
+  int o_by_32;                      // rows of O start on 32-byte boundaries
   int box;                          // rows of a TMA box: 32 where a page is a multiple of that, else 16
   float scale_log2;
   float* part_o;                    // [grid][2][WARPS][NQ D / 4][32 lanes]
@@ -146,6 +149,12 @@ template <int ROWS> struct Cursor {
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
+// 16 bytes, or sixteen zero bytes without a look at the source
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
+  const int bytes = take ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // an arrival on `bar` (counted in its initial count) once this thread's cp.async so far have landed
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -155,6 +164,10 @@ __device__ __forceinline__ void lds128(uint32_t addr, uint32_t (&r)[4]) {
 }
 __device__ __forceinline__ void lds64(uint32_t addr, uint32_t (&r)[2]) {
   asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr));
+}
+
+__device__ __forceinline__ void sts128(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
 }
 
 // The low / high two e4m3 codes of a word as two f16.
@@ -1089,6 +1102,7 @@ extern "C" int kcg_fmha_cached_fwd(int dtype, int64_t T, int64_t B, int64_t Hq, 
   p.B = static_cast<int>(B); p.Hkv = static_cast<int>(Hkv); p.G = static_cast<int>(Hq / Hkv);
   p.page = static_cast<int>(page_size); p.causal = causal != 0;
   p.box = page_size % 32 == 0 ? 32 : 16;
+  p.o_by_32 = (reinterpret_cast<uintptr_t>(O) & 31u) == 0 && o_strides[0] % 16 == 0 && o_strides[1] % 16 == 0;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.status = device_status_word();
   cudaStream_t s = static_cast<cudaStream_t>(stream);

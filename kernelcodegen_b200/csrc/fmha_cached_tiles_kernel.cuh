@@ -1,13 +1,18 @@
 // Attention over the paged 8-bit cache for many query rows per request (included by fmha_cached.cu inside its anonymous
-// namespace).  Here the two matrix products are the cost, so they run on tcgen05 with 128-row tiles:
+// namespace).  Here the two matrix products are the cost, so they run on tcgen05 with 128-row tiles, in the order of the
+// two-tile kernel of fmha_tcgen05.cu:
 //
 //   An item is a pair of 128-row tiles of one (request, key / value head): rows are (token, query head of the group) in
 //   token-major order, so a block of 128 keys is loaded and converted once for 256 rows, whatever the group.
 //   warps 0-3, 4-7  softmax of tile 0 / 1, one thread per row (scores, P and O in tensor memory); before that, the row
 //                   of Q, as f16 scaled by a power of two, into the swizzled tile the products read; afterwards, O out
 //   warp 8          one thread issues the products: S_i = Q_i K^T, O_i += P_i V, S_i(j + 1) right behind P_i V(j)
-//   warp 9          looks pages up and loads the codes of K and V by TMA (boxes of 16 or 32 rows of a page)
-//   warps 12-15     turn codes into f16 tiles in the swizzled layout tcgen05 wants (the same for K and V)
+//   warp 9          walks the items, looks pages and scales up (a record per key block) and loads the codes of K and V by
+//                   TMA (boxes of 16 or 32 rows of a page)
+//   warps 10-15     turn codes into f16 tiles in the swizzled layout tcgen05 wants, the same for K and V
+// Every ring and barrier runs on across items: records, codes and the first tiles of the next item are on their way while
+// the last blocks of this one are worked on.
+//
 // tcgen05 multiplies f16 with f16 or e4m3 with e4m3, not one with the other, and P in e4m3 would keep four bits; so the
 // codes are widened on the way.  Scales: a page's is 2^e f with f in [1, 2).  The power of two, relative to the block's
 // largest (K) or the item's largest so far (V), is multiplied into the codes, exactly down to f16's smallest step (a
@@ -17,33 +22,40 @@
 // Tensor memory (512 columns): S0, S1, O0, O1; P_i overwrites the first half of S_i.
 #pragma once
 
-constexpr int TM = 128;                 // rows of a tile
-constexpr int TN = 128;                 // keys of a block
-constexpr int TILES_THREADS = 512;
-constexpr int TILES_REGS_SOFTMAX = 200, TILES_REGS_OTHER = 56;
+constexpr int TM = 128;                 // rows of a tile; BN keys of a block
+constexpr int TILES_THREADS = 512, CONVERT_WARPS = 6;
+constexpr int TILES_REGS_SOFTMAX = 184, TILES_REGS_OTHER = 72;
 static_assert(2 * 128 * (TILES_REGS_SOFTMAX + TILES_REGS_OTHER) <= TILES_THREADS * 128, "register split exceeds the block's allocation");
-constexpr int RECORDS = 8;
+// A record is written when the codes of the K tile before it have been converted, which is at most two blocks (the ring of f16
+// tiles) before the softmax is through with that block: it is read at most four blocks after it is written.
+constexpr int RECORDS = 6, ITEMS = 4;
 
-// What the loader says about a key block.
+// What the look-up says about a key block.
 struct BlockRecord {
   float kref;                           // scores are to be multiplied with this
   float vshift;                         // what the output so far is to be multiplied with (V's reference has grown)
   float vref;                           // V's reference
   int plain;                            // every group's page is there, every f of K is 1
+  uint32_t gone;                        // groups whose page is not in the pool: their keys are left out
+  int have;                             // keys up to the request's last token; -1: there is no block and none will come
+  int mode[2];                          // of K, V: 0: codes become f16 as they are, 1: times a power of two, 2: there is more to it
   uint32_t rk[8], rv[8];                // per group of 16 keys: what its codes are multiplied with, two f16
   float fk[8], fv[8];                   // f
-  uint32_t gone;                        // groups whose page is not in the pool: their keys are left out
+};
+struct TilesItem {
+  int t0, n, len, head, row0, go;       // the request's first row of Q, rows, keys; key head; first row of the pair
+  int pad[2];
 };
 
 template <int D> struct TilesSmem {
   static constexpr int DB = D / 64;
   static constexpr int TILE = DB * 16384;               // bytes of a 128 x D f16 tile: DB blocks of 128 rows x 128 bytes
   uint8_t q[2][TILE], k[2][TILE], v[2][TILE];
-  uint8_t raw[2][TN * D];                               // codes of K, V
+  uint8_t raw[2][BN * D];                               // codes of K, V, as TMA's swizzle leaves them
   BlockRecord rec[RECORDS];
-  uint64_t raw_full[2], raw_empty[2], k_full[2], k_empty[2], v_full[2], v_empty[2], rec_full[RECORDS];
+  TilesItem item[ITEMS];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], rec_full[RECORDS], raw_full[2], raw_empty[2], item_full[ITEMS], item_empty[ITEMS];
   uint64_t q_full, s_full[2], p_full[4], o_full[2], drain;
-  int item[8];                                          // t0, n, len, head, pair, go
   uint32_t tmem;
   int abort;
 };
@@ -58,13 +70,128 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-__device__ __forceinline__ float max3f(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
+// pv4_peek with a second barrier tested along.
+__device__ __forceinline__ bool pv4_peek2(uint32_t d_o, uint32_t a_p, uint64_t vd, uint32_t idesc, uint32_t acc_first, uint32_t peek1,
+                                          uint32_t par1, uint32_t peek2, uint32_t par2, bool& ok2) {
+  uint32_t r1, r2;
+  asm volatile(
+      "{\n\t.reg .pred P, Q1, Q2, T;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 v1, v2, v3;\n\t"
+      "setp.ne.b32 P, %6, 0;\n\t"
+      "setp.eq.b32 T, %6, %6;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 Q1, [%7], %8;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 Q2, [%9], %10;\n\t"
+      "add.u32 a1, %3, 8;\n\tadd.u32 a2, %3, 16;\n\tadd.u32 a3, %3, 24;\n\t"
+      "add.s64 v1, %4, 128;\n\tadd.s64 v2, %4, 256;\n\tadd.s64 v3, %4, 384;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%2], [%3], %4, %5, P;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%2], [a1], v1, %5, T;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%2], [a2], v2, %5, T;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%2], [a3], v3, %5, T;\n\t"
+      "selp.u32 %0, 1, 0, Q1;\n\tselp.u32 %1, 1, 0, Q2;\n\t}"
+      : "=r"(r1), "=r"(r2)
+      : "r"(d_o), "r"(a_p), "l"(vd), "r"(idesc), "r"(acc_first), "r"(peek1), "r"(par1), "r"(peek2), "r"(par2)
+      : "memory");
+  ok2 = r2 != 0;
+  return r1 != 0;
 }
 
-// Items of a request; the longest (under a causal mask the last rows) come first.
+// The online softmax of one key block for the calling thread's row, as softmax_block does it, but holding 64 scores at a time:
+// with half of the warps converting, 128 scores and their helpers (about 210 registers) do not fit the softmax warps.
+// Scores are read again from tensor memory where both halves are needed twice.
+template <int D, typename Arrive>
+__device__ __forceinline__ void softmax_halves(uint32_t s_addr, uint32_t o_addr, int j, int limit, float c, float& m, float& l, int lane,
+                                               Arrive arrive) {
+  const uint64_t c2 = f2_pack(c, c);
+  uint64_t sum_a = 0ull, sum_b = 0ull;
+  uint32_t s[64], pk[32];
+  auto load = [&](int half) {
+    tmem_ld64(s_addr + 64 * half, s);
+    tmem_wait_ld();
+    if (limit < BN) {
+#pragma unroll
+      for (int k = 0; k < 64; ++k)
+        if (64 * half + k >= limit) s[k] = 0xff800000u;
+    }
+  };
+  auto maximum = [&]() {
+    float mx[4];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) mx[a] = fmaxf(__uint_as_float(s[2 * a]), __uint_as_float(s[2 * a + 1]));
+#pragma unroll
+    for (int k = 8; k < 64; k += 8)
+#pragma unroll
+      for (int a = 0; a < 4; ++a) mx[a] = max3(mx[a], __uint_as_float(s[k + 2 * a]), __uint_as_float(s[k + 2 * a + 1]));
+    return fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
+  };
+  auto exponentials = [&](float base) {
+    const uint64_t nb2 = f2_pack(-base, -base);
+#pragma unroll
+    for (int k = 0; k < 64; k += 2) {
+      float x0, x1;
+      f2_unpack(f2_fma(f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c2, nb2), x0, x1);
+      const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+      if ((k >> 1) & 1) sum_b = f2_add(sum_b, f2_pack(p0, p1));
+      else sum_a = f2_add(sum_a, f2_pack(p0, p1));
+      pk[k >> 1] = pack2<__half>(p0, p1);
+    }
+  };
+  auto hand_over = [&](int half) {
+    tmem_st32(s_addr + half * 32, pk);
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) arrive(half);
+  };
+  float alpha = 1.f;
+  bool done = false;
+  // Speculation, as in softmax_block: the first half's exponentials with the maximum so far, before this block's is known.
+  if (__all_sync(0xffffffffu, j > 0 && limit >= BN && m != -INFINITY)) {
+    load(0);
+    exponentials(m);
+    float mt = maximum();
+    load(1);
+    mt = fmaxf(mt, maximum()) * c;
+    if (!__any_sync(0xffffffffu, mt > m + kLazy)) {
+      hand_over(0);
+      exponentials(m);
+      hand_over(1);
+      done = true;
+    } else {
+      sum_a = sum_b = 0ull;
+    }
+  }
+  if (!done) {
+    load(0);
+    float mt = maximum();
+    load(1);
+    mt = fmaxf(mt, maximum()) * c;
+    if (mt > m + kLazy) {
+      alpha = fast_exp2(m - mt);            // 0 for the row's first keys
+      m = mt;
+    }
+    if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll 1
+      for (int cc = 0; cc < D / 32; ++cc) {
+        tmem_ld32(o_addr + cc * 32, pk);
+        tmem_wait_ld();
+#pragma unroll
+        for (int k = 0; k < 32; ++k) pk[k] = __float_as_uint(__uint_as_float(pk[k]) * alpha);
+        tmem_st32(o_addr + cc * 32, pk);
+        tmem_wait_st();                     // (the registers of a store are not touched before it is done)
+      }
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    load(0);
+    exponentials(base);
+    hand_over(0);
+    load(1);
+    exponentials(base);
+    hand_over(1);
+  }
+  float l0, l1;
+  f2_unpack(f2_add(sum_a, sum_b), l0, l1);
+  l = l * alpha + (l0 + l1);
+}
+
 __device__ __forceinline__ int64_t request_items(const CachedParams& p, const Request& r) {
   return static_cast<int64_t>(p.Hkv) * ((r.n * p.G + 2 * TM - 1) / (2 * TM));
 }
@@ -84,10 +211,10 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     prefetch_tmap(&tmV);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sm.raw_full[s], 1);
-      mbar_init(&sm.raw_empty[s], 4);
-      mbar_init(&sm.k_full[s], 4);
+      mbar_init(&sm.raw_empty[s], CONVERT_WARPS);
+      mbar_init(&sm.k_full[s], CONVERT_WARPS);
       mbar_init(&sm.k_empty[s], 1);
-      mbar_init(&sm.v_full[s], 4);
+      mbar_init(&sm.v_full[s], CONVERT_WARPS);
       mbar_init(&sm.v_empty[s], 1);
       mbar_init(&sm.s_full[s], 1);
       mbar_init(&sm.o_full[s], 1);
@@ -95,6 +222,10 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       mbar_init(&sm.p_full[2 * s + 1], 4);
     }
     for (int s = 0; s < RECORDS; ++s) mbar_init(&sm.rec_full[s], 1);
+    for (int s = 0; s < ITEMS; ++s) {
+      mbar_init(&sm.item_full[s], 1);
+      mbar_init(&sm.item_empty[s], 9);      // eight softmax warps and the issuing thread
+    }
     mbar_init(&sm.q_full, 8);
     mbar_init(&sm.drain, 1);
     sm.abort = 0;
@@ -114,134 +245,123 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       if (p.status) *p.status = KCG_ERR_TIMEOUT;
     }
   };
+  // key blocks of the tile of rows that begins at `first`: up to the last key its last row sees
+  auto blocks_of = [&](int first, int n, int len) {
+    const int last = min(first + TM, n * p.G) - 1;
+    if (last < first) return 0;
+    const int end = p.causal ? min(len, len - n + 1 + last / p.G) : len;
+    return end > 0 ? (end + BN - 1) / BN : 0;
+  };
 
-  // Items are dealt round-robin.  All warps meet before and behind an item (every wait in between is bounded, so every
-  // warp gets there); the loader's first thread walks the requests.
-  auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(TILES_THREADS) : "memory"); };
-  int64_t left = blockIdx.x;              // items between the walk's place and this block's next item
-  int walk_i = 0;
-  auto find_item = [&]() {
-    bool go = false;
-    Request r{0, 0, 0};
-    for (; walk_i < p.B; ++walk_i) {
-      r = request_of(p, walk_i);
-      const int64_t n = request_items(p, r);
-      if (left < n) {
-        go = true;
-        break;
-      }
-      left -= n;
-    }
-    sm.item[5] = go;
-    if (go) {
-      const int pairs = (r.n * p.G + 2 * TM - 1) / (2 * TM);
-      const int idx = static_cast<int>(left);
-      sm.item[0] = r.t0;
-      sm.item[1] = r.n;
-      sm.item[2] = r.len;
-      sm.item[3] = idx / pairs;
-      sm.item[4] = pairs - 1 - idx % pairs;
-      sm.item[6] = walk_i;
-      left += gridDim.x;
-    }
-  };
-  uint32_t blocks = 0;                    // key blocks done before this item (phases of the rings and records)
-  struct Item {
-    int t0, n, len, head, row0, req, rows, n0, n1, nmax;
-  };
-  auto begin_item = [&](Item& it) {
-    meet();
-    if (!sm.item[5] || *abort_flag) return false;
-    it.t0 = sm.item[0];
-    it.n = sm.item[1];
-    it.len = sm.item[2];
-    it.head = sm.item[3];
-    it.row0 = sm.item[4] * 2 * TM;
-    it.req = sm.item[6];
-    it.rows = it.n * p.G;
-    // key blocks of the two tiles: up to the last key their last row sees
-    auto blocks_of = [&](int first) {
-      const int last = min(first + TM, it.rows) - 1;
-      if (last < first) return 0;
-      const int end = p.causal ? min(it.len, it.len - it.n + 1 + last / p.G) : it.len;
-      return end > 0 ? (end + TN - 1) / TN : 0;
+  if (warp < 8) {
+    // ------------------------------------------------------------------ softmax
+    reg_alloc<TILES_REGS_SOFTMAX>();
+    const int i = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    // (Registers are what this role is short of: an item's description stays in shared memory until its output is out.)
+    const uint32_t s_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + i * BN, o_addr = s_addr + 256;
+    static_assert(BN == TM, "O_i stands 256 columns behind S_i");
+    uint32_t b = 0, phases = 0;             // key block; phases of s_full (bit 0) and o_full (bit 1)
+    // Rows of Q and O cross global memory whole: PPR lanes with 16 bytes each take a row, RPI rows at a time.
+    constexpr int PPR = D / 8, RPI = 32 / PPR;
+    // A thread works out where its own row is (a division) and the others ask it.
+    auto offset_of = [&](const TilesItem& it, int64_t by_token, int64_t by_head) -> int64_t {   // -1: not a row
+      const int R = it.row0 + i * TM + r;
+      if (R >= it.n * p.G) return -1;
+      const int token = R / p.G;
+      return (it.t0 + token) * by_token + (it.head * p.G + R - token * p.G) * by_head;
     };
-    it.n0 = blocks_of(it.row0);
-    it.n1 = blocks_of(it.row0 + TM);
-    it.nmax = max(it.n0, it.n1);
-    return true;
-  };
-
-    if (warp < 8) {
-      // ------------------------------------------------------------------ softmax
-      reg_alloc<TILES_REGS_SOFTMAX>();
-      uint32_t cs = 0, cf = 0;              // score tiles and outputs of this tile so far
-      Item it;
-      while (begin_item(it)) {
-      const int t0 = it.t0, n = it.n, len = it.len, head = it.head, row0 = it.row0, rows = it.rows;
-      const int i = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
-      const int R = row0 + i * TM + r;
-      const bool live = R < rows;
-      const int j_row = live ? R / p.G : 0;
-      const int64_t q_at = (t0 + j_row) * p.q_st + (head * p.G + (live ? R - j_row * p.G : 0)) * p.q_sh;
-      float c = fabsf(p.scale_log2);
-      {
-        // this thread's row of Q: in two passes, largest magnitude, then f16
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.Q) + q_at);
-        float up = p.scale_log2 < 0.f ? -1.f : 1.f;      // the softmax's constant is not negative
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          uint32_t m = 0;
-          if (live)
+    // The warp's 32 rows of Q: fetched as they are, straight to where they will be read, and turned into f16 there, every
+    // thread its own row.  Returns what the row's scores are to be multiplied with.
+    auto fetch_q = [&](const TilesItem& it) {
+      const int64_t mine = offset_of(it, p.q_st, p.q_sh);
 #pragma unroll
-            for (int k = 0; k < D / 8; ++k) {
-              const uint4 x = __ldg(src + k);
-              m = __vmaxu2(__vmaxu2(__vmaxu2(__vmaxu2(m, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu), x.z & 0x7fff7fffu), x.w & 0x7fff7fffu);
-            }
-          m = max(m & 0xffffu, m >> 16);
-          int e = static_cast<int>(m >> 7) - 127 - 13;
-          e = e < -113 ? -113 : e;
-          up *= __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-          c *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-        }
-#pragma unroll
-        for (int k = 0; k < D / 8; ++k) {
-          const uint4 x = live ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-          uint32_t h[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float f[2];
-            Words<T>::unpack(w[e], f);
-            h[e] = pack_f16(f[0] * up, f[1] * up);
-          }
-          *reinterpret_cast<uint4*>(sm.q[i] + (k >> 3) * 16384 + r * 128 + (((k & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.q_full);
+      for (int k = 0; k < 32 / RPI; ++k) {
+        const int64_t at = __shfl_sync(0xffffffffu, mine, k * RPI + lane / PPR);
+        const int row = quarter * 32 + k * RPI + lane / PPR, ch = lane % PPR;
+        cp_async16(smem_u32(sm.q[i]) + (ch >> 3) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4),
+                   static_cast<const T*>(p.Q) + max(at, static_cast<int64_t>(0)) + ch * 8, at >= 0);
       }
-      const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-      const uint32_t s_addr = tmem + lane_base + i * TN, o_addr = tmem + lane_base + 256 + i * TM;
-      const int n_mine = i == 0 ? it.n0 : it.n1;
-      const int end = live ? (p.causal ? min(len, len - n + 1 + j_row) : len) : 0;   // keys this row sees
-      float m = -INFINITY, l = 0.f, vref = 1.f;
-      bool ok = true;
-      for (int j = 0; j < n_mine; ++j, ++cs) {
-        const BlockRecord& rec = sm.rec[(blocks + j) % RECORDS];
-        if (!mbar_wait(&sm.rec_full[(blocks + j) % RECORDS], ((blocks + j) / RECORDS) & 1u, abort_flag) ||
-            !mbar_wait(&sm.s_full[i], cs & 1u, abort_flag)) {
-          ok = false;
-          break;
+    };
+    auto convert_q = [&]() -> float {
+      cp_async_wait_all();
+      __syncwarp();                         // (a thread's row was fetched by its neighbours)
+      const uint32_t row = smem_u32(sm.q[i]) + r * 128;
+      auto piece = [&](int k) { return row + (k >> 3) * 16384 + (((k & 7) ^ (r & 7)) << 4); };
+      const bool negative = p.scale_log2 < 0.f;          // the softmax's constant is not negative
+      float factor = 1.f;
+      if (std::is_same<T, __nv_bfloat16>::value || negative) {
+        uint32_t w[PPR][4];
+#pragma unroll
+        for (int k = 0; k < PPR; ++k) lds128(piece(k), w[k]);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          uint32_t big = 0;
+#pragma unroll
+          for (int k = 0; k < PPR; ++k)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) big = __vmaxu2(big, w[k][x] & 0x7fff7fffu);
+          big = max(big & 0xffffu, big >> 16);
+          int e = static_cast<int>(big >> 7) - 127 - 13;  // largest element to [2^13, 2^14)
+          e = e < -113 ? -113 : e;
+          const float up = __uint_as_float((static_cast<uint32_t>(127 - e) << 23) | (negative ? 0x80000000u : 0u));
+          factor = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+#pragma unroll
+          for (int k = 0; k < PPR; ++k)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) w[k][x] = pack_f16(__uint_as_float(w[k][x] << 16) * up, __uint_as_float(w[k][x] & 0xffff0000u) * up);
+        } else {
+#pragma unroll
+          for (int k = 0; k < PPR; ++k)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) w[k][x] ^= 0x80008000u;
         }
-        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < PPR; ++k) sts128(piece(k), w[k]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.q_full);
+      return factor * fabsf(p.scale_log2);
+    };
+    bool ok = true, have_q = false;
+    float c = 0.f;
+    for (uint32_t k_item = 0; ok; ++k_item) {
+      if (!mbar_wait(&sm.item_full[k_item % ITEMS], (k_item / ITEMS) & 1u, abort_flag)) { ok = false; break; }
+      const TilesItem& it = sm.item[k_item % ITEMS];
+      if (!it.go) break;
+      // key blocks of this tile and of the other; keys this row sees from block b on
+      const int n_mine = blocks_of(it.row0 + i * TM, it.n, it.len), n_other = blocks_of(it.row0 + (1 - i) * TM, it.n, it.len);
+      int seen = 0;
+      {
+        const int R = it.row0 + i * TM + r;
+        if (R < it.n * p.G) seen = p.causal ? min(it.len, it.len - it.n + 1 + R / p.G) : it.len;
+      }
+      if (!have_q) {
+        fetch_q(it);
+        c = convert_q();
+      }
+      have_q = false;
+      float m = -INFINITY, l = 0.f, vref = 1.f;
+      for (int j = 0; j < n_mine; ++j, ++b, phases ^= 1u) {
+        const BlockRecord& rec = sm.rec[b % RECORDS];
+        if (!mbar_wait(&sm.rec_full[b % RECORDS], (b / RECORDS) & 1u, abort_flag)) { ok = false; break; }
         float cj = c * rec.kref;
-        const bool plain = rec.plain != 0;
+        const bool odd = __any_sync(0xffffffffu, rec.plain == 0 || cj == 0.f);
         const float vshift = rec.vshift;
         vref = rec.vref;
-        if (__any_sync(0xffffffffu, !plain || cj == 0.f)) {
+        if (!mbar_wait(&sm.s_full[i], phases & 1u, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        if (j + 1 == n_mine) {
+          // the tile's last scores are there, so its Q is free: the next item's, if that is known already
+          const uint32_t next = k_item + 1;
+          if (__all_sync(0xffffffffu, mbar_try_wait(&sm.item_full[next % ITEMS], (next / ITEMS) & 1u)) && sm.item[next % ITEMS].go) {
+            fetch_q(sm.item[next % ITEMS]);
+            have_q = true;
+          }
+        }
+        if (odd) {
           // scores that a block-wide constant does not serve are put right in place, in pieces that leave registers alone
 #pragma unroll 1
-          for (int cc = 0; cc < TN / 32; ++cc) {
+          for (int cc = 0; cc < BN / 32; ++cc) {
             uint32_t x[32];
             tmem_ld32(s_addr + cc * 32, x);
             tmem_wait_ld();
@@ -251,81 +371,36 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
               x[k] = (rec.gone >> (2 * cc + (k >> 4))) & 1u ? 0xff800000u : __float_as_uint(__uint_as_float(x[k]) * f);
             }
             tmem_st32(s_addr + cc * 32, x);
+            tmem_wait_st();
           }
-          tmem_wait_st();
           if (cj == 0.f) cj = 1.f;                       // (-inf times 0 is not -inf)
         }
-        uint32_t s[TN];
-        tmem_ld64(s_addr, reinterpret_cast<uint32_t(&)[64]>(s[0]));
-        tmem_ld64(s_addr + 64, reinterpret_cast<uint32_t(&)[64]>(s[64]));
-        tmem_wait_ld();
-        const int limit = end - j * TN;
-        if (limit < TN) {
-#pragma unroll
-          for (int k = 0; k < TN; ++k)
-            if (k >= limit) s[k] = 0xff800000u;
-        }
-        float mx[8];
-#pragma unroll
-        for (int a = 0; a < 8; ++a) mx[a] = fmaxf(__uint_as_float(s[2 * a]), __uint_as_float(s[2 * a + 1]));
-#pragma unroll
-        for (int k = 16; k < TN; k += 16)
-#pragma unroll
-          for (int a = 0; a < 8; ++a) mx[a] = max3f(mx[a], __uint_as_float(s[k + 2 * a]), __uint_as_float(s[k + 2 * a + 1]));
-        const float top = max3f(max3f(mx[0], mx[1], mx[2]), max3f(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
-        const float mt = top * cj;
-        float alpha = 1.f;
-        if (mt > m + kLazy) {
-          alpha = exp2f_approx(m - mt);                  // 0 for the first keys
-          m = mt;
-        }
         // the scores being complete means that P V of the block before is, too: O may be changed
-        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f || vshift != 1.f)) {
-          const float a = alpha * vshift;
+        if (j > 0 && vshift != 1.f) {
 #pragma unroll 1
           for (int cc = 0; cc < D / 32; ++cc) {
             uint32_t x[32];
             tmem_ld32(o_addr + cc * 32, x);
             tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * a);
+            for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * vshift);
             tmem_st32(o_addr + cc * 32, x);
+            tmem_wait_st();
           }
-          tmem_wait_st();
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        const uint64_t c2 = pk_make(cj, cj), nb2 = pk_make(-base, -base);
-        uint64_t sum_a = 0ull, sum_b = 0ull;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-#pragma unroll
-          for (int k = half * 64; k < half * 64 + 64; k += 2) {
-            float x0, x1;
-            pk_split(pk_fma(pk_make(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c2, nb2), x0, x1);
-            float p0 = exp2f_approx(x0), p1 = exp2f_approx(x1);
-            if ((k >> 1) & 1) sum_b = pk_add(sum_b, pk_make(p0, p1));
-            else sum_a = pk_add(sum_a, pk_make(p0, p1));
-            s[k >> 1] = pack_f16(p0, p1);                // word k / 2 is not read again
-          }
-          tmem_st32(s_addr + half * 32, reinterpret_cast<uint32_t(&)[32]>(s[half * 32]));
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.p_full[2 * i + half]);
-        }
-        float l0, l1;
-        pk_split(pk_add(sum_a, sum_b), l0, l1);
-        l = l * alpha + (l0 + l1);
+        softmax_halves<D>(s_addr, o_addr, j, seen - j * BN, cj, m, l, lane, [&](int half) { mbar_arrive(&sm.p_full[2 * i + half]); });
       }
+      // The next item's scores may be computed while this one's output leaves.
+      if (ok && have_q) c = convert_q();
       if (ok && n_mine > 0) {
-        ok = mbar_wait(&sm.o_full[i], cf & 1u, abort_flag);
-        ++cf;
+        ok = mbar_wait(&sm.o_full[i], phases >> 1, abort_flag);
+        phases ^= 2u;
         tc_fence_after();
       }
-      if (!ok) give_up();
-      if (ok) {
+      if (!ok) break;
+      {
         const float inv = l == 0.f ? 0.f : vref / l;     // a row that sees no key is zero
-        T* dst = static_cast<T*>(p.O) + (t0 + j_row) * p.o_st + (head * p.G + (live ? R - j_row * p.G : 0)) * p.o_sh;
+        const int64_t at = offset_of(it, p.o_st, p.o_sh);
 #pragma unroll 1
         for (int cc = 0; cc < D / 32; ++cc) {
           uint32_t x[32];
@@ -333,115 +408,163 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             tmem_ld32(o_addr + cc * 32, x);
             tmem_wait_ld();
           }
-          if (live) {
+          uint4 w[4];
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              uint32_t w[4];
+          for (int k = 0; k < 16; ++k) {
+            const float f[2] = {__uint_as_float(x[2 * k]) * inv, __uint_as_float(x[2 * k + 1]) * inv};
+            reinterpret_cast<uint32_t*>(w)[k] = l == 0.f ? 0u : Words<T>::pack(f);
+          }
+          if (at >= 0) {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.O) + at + cc * 32);
+            if (p.o_by_32) {                // whole sectors
+              st_256(dst, w[0], w[1]);
+              st_256(dst + 2, w[2], w[3]);
+            } else {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float f[2] = {l == 0.f ? 0.f : __uint_as_float(x[k + 2 * e]) * inv, l == 0.f ? 0.f : __uint_as_float(x[k + 2 * e + 1]) * inv};
-                w[e] = Words<T>::pack(f);
-              }
-              *reinterpret_cast<uint4*>(dst + cc * 32 + k) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int k = 0; k < 4; ++k) dst[k] = w[k];
             }
           }
         }
-        tc_fence_before();
+        tc_fence_before();                  // (the next item's first product overwrites O behind this thread's first P)
       }
-      blocks += it.nmax;
-      meet();
-      }
-    } else if (warp == 8) {
-      // ------------------------------------------------------------------ products
-      reg_dealloc<TILES_REGS_OTHER>();
-      uint32_t items = 0, cp0 = 0, cp1 = 0; // items, P blocks of the tiles so far
-      Item it;
-      while (begin_item(it)) {
-      const int n0 = it.n0, n1 = it.n1, nmax = it.nmax;
-      if (lane == 0) {
-        bool ok = mbar_wait(&sm.q_full, items & 1u, abort_flag);
-        ++items;
-        const uint64_t qd = make_smem_desc(smem_u32(sm.q[0]), 16, 1024), kd = make_smem_desc(smem_u32(sm.k[0]), 16, 1024);
-        const uint64_t vd = make_smem_desc(smem_u32(sm.v[0]), 16384, 1024);
-        auto scores = [&](int i, uint32_t slot) {
-#pragma unroll
-          for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_ss<Kind::F16>(tmem + i * TN, qd + ((i * TILE + d * 16384 + k * 32) >> 4), kd + ((slot * TILE + d * 16384 + k * 32) >> 4),
-                                idesc_qk, (d | k) != 0 ? 1u : 0u);
-          mma_commit(&sm.s_full[i]);
-        };
-        auto output = [&](int i, int half, uint32_t slot, uint32_t first) {
-#pragma unroll
-          for (int k = 4 * half; k < 4 * half + 4; ++k)
-            mma_ts_f16(tmem + 256 + i * TM, tmem + i * TN + k * 8, vd + ((slot * TILE + k * 2048) >> 4), idesc_pv, (first | k) != 0 ? 1u : 0u);
-        };
-        if (ok && nmax > 0) {
-          ok = mbar_wait(&sm.k_full[blocks & 1u], (blocks >> 1) & 1u, abort_flag);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.item_empty[k_item % ITEMS]);
+      b += max(n_other - n_mine, 0);
+    }
+    if (!ok) give_up();
+  } else if (warp == 8) {
+    // ------------------------------------------------------------------ products
+    reg_dealloc<TILES_REGS_OTHER>();
+    if (lane == 0) {
+      const uint64_t qd = make_smem_desc(smem_u32(sm.q[0]), 16, 1024), kd = make_smem_desc(smem_u32(sm.k[0]), 16, 1024);
+      const uint64_t vd = make_smem_desc(smem_u32(sm.v[0]), 16384, 1024);
+      const uint32_t kf = smem_u32(sm.k_full), vf = smem_u32(sm.v_full), pf = smem_u32(sm.p_full), sf = smem_u32(sm.s_full),
+                     of = smem_u32(sm.o_full);
+      uint32_t blocks = 0, cp0 = 0, cp1 = 0;             // key blocks before this item, P blocks of the tiles so far
+      bool ok = true;
+      for (uint32_t k_item = 0; ok; ++k_item) {
+        if (!mbar_wait(&sm.item_full[k_item % ITEMS], (k_item / ITEMS) & 1u, abort_flag)) { ok = false; break; }
+        const TilesItem it = sm.item[k_item % ITEMS];
+        mbar_arrive(&sm.item_empty[k_item % ITEMS]);
+        if (!it.go) break;
+        const int n0 = blocks_of(it.row0, it.n, it.len), n1 = blocks_of(it.row0 + TM, it.n, it.len), nmax = max(n0, n1);
+        if (!mbar_wait(&sm.q_full, k_item & 1u, abort_flag)) { ok = false; break; }
+        if (nmax > 0) {
+          if (!mbar_wait(&sm.k_full[blocks & 1u], (blocks >> 1) & 1u, abort_flag)) { ok = false; break; }
           tc_fence_after();
-          if (ok) {
-            if (n0 > 0) scores(0, blocks & 1u);
-            if (n1 > 0) scores(1, blocks & 1u);
-            mma_commit(&sm.k_empty[blocks & 1u]);
-          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            if ((i == 0 ? n0 : n1) > 0) {
+#pragma unroll
+              for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  mma_ss<Kind::F16>(tmem + i * BN, qd + ((i * TILE + d * 16384 + k * 32) >> 4),
+                                    kd + (((blocks & 1u) * TILE + d * 16384 + k * 32) >> 4), idesc_qk, (d | k) != 0 ? 1u : 0u);
+              mma_commit(&sm.s_full[i]);
+            }
+          mma_commit(&sm.k_empty[blocks & 1u]);
         }
+        // barriers already seen complete by a test that rode along with an earlier batch of products
+        bool r_v = false, r_p00 = false, r_p10 = false;
         for (int j = 0; j < nmax && ok; ++j) {
-          const uint32_t b = blocks + j, slot = b & 1u, next = (b + 1) & 1u;
-          ok = mbar_wait(&sm.v_full[slot], (b >> 1) & 1u, abort_flag);
-          bool k_ready = false;
+          const uint32_t b = blocks + j, slot = b & 1u, next = slot ^ 1u;
+          if (!r_v && !mbar_wait(&sm.v_full[slot], (b >> 1) & 1u, abort_flag)) { ok = false; break; }
+          r_v = false;
+          bool r_k = false;
+          const uint64_t v = vd + ((slot * TILE) >> 4), k = kd + ((next * TILE) >> 4);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int n_i = i == 0 ? n0 : n1;
-            if (!ok || j >= n_i) continue;
+            if (j >= n_i) continue;
             uint32_t& cp = i == 0 ? cp0 : cp1;
-            if (!mbar_wait(&sm.p_full[2 * i], cp & 1u, abort_flag)) { ok = false; break; }
+            bool& r_p = i == 0 ? r_p00 : r_p10;
+            const uint32_t pj = cp & 1u;
+            if (!r_p && !mbar_wait(&sm.p_full[2 * i], pj, abort_flag)) { ok = false; break; }
+            r_p = false;
             tc_fence_after();
-            output(i, 0, slot, j);
-            if (!mbar_wait(&sm.p_full[2 * i + 1], cp & 1u, abort_flag)) { ok = false; break; }
-            tc_fence_after();
-            output(i, 1, slot, j);
+            const uint32_t d_o = tmem + 256 + i * TM, a_p = tmem + i * BN;
+            bool seen_k;
+            const bool seen_p = pv4_peek2(d_o, a_p, v, idesc_pv, j != 0 ? 1u : 0u, pf + (2 * i + 1) * 8, pj, kf + next * 8, ((b + 1) >> 1) & 1u, seen_k);
+            if (!seen_p && !mbar_wait(&sm.p_full[2 * i + 1], pj, abort_flag)) { ok = false; break; }
             ++cp;
+            bool t1, t2;
+            // tested meanwhile: behind tile 0 the first half of tile 1's P, behind tile 1 the next V and tile 0's next P
+            const uint32_t peek1 = i == 0 ? pf + 2 * 8 : vf + next * 8, par1 = i == 0 ? (cp1 & 1u) : (((b + 1) >> 1) & 1u);
+            const uint32_t peek2 = pf, par2 = cp0 & 1u;
+            const uint64_t q = qd + ((i * TILE) >> 4);
             if (j + 1 < n_i) {
-              if (!k_ready && !mbar_wait(&sm.k_full[next], ((b + 1) >> 1) & 1u, abort_flag)) { ok = false; break; }
-              k_ready = true;
+              if (!r_k && !seen_k && !mbar_wait(&sm.k_full[next], ((b + 1) >> 1) & 1u, abort_flag)) { ok = false; break; }
+              r_k = true;
               tc_fence_after();
-              scores(i, next);
+              pv4_s_commit_peek2<D, true>(d_o, a_p + 32, v + 512, idesc_pv, tmem + i * BN, q, k, idesc_qk, sf + i * 8, peek1, par1, peek2, par2, t1, t2);
             } else {
-              mma_commit(&sm.o_full[i]);
+              tc_fence_after();
+              pv4_s_commit_peek2<D, false>(d_o, a_p + 32, v + 512, idesc_pv, tmem + i * BN, q, k, idesc_qk, of + i * 8, peek1, par1, peek2, par2, t1, t2);
+            }
+            if (i == 0) {
+              r_p10 = t1 && j < n1;
+            } else {
+              r_v = t1 && j + 1 < nmax;
+              r_p00 = t2 && j + 1 < n0;
             }
           }
           if (!ok) break;
           mma_commit(&sm.v_empty[slot]);
           if (j + 1 < nmax) mma_commit(&sm.k_empty[next]);
         }
-        if (!ok) {
-          give_up();
-          int zero = 0;
-          mma_commit(&sm.drain);          // what was issued must end before the block does
-          mbar_wait(&sm.drain, 0, &zero, 20000000ull);
+        blocks += nmax;
+      }
+      if (!ok) give_up();
+      int zero = 0;
+      mma_commit(&sm.drain);                // what was issued must end before the block does
+      mbar_wait(&sm.drain, 0, &zero, 20000000ull);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------ items, pages, scales
+    // Items are dealt round-robin, the last rows of a head (under a causal mask the longest) first.  Lane g < 8 looks after
+    // a block's keys 16 g .. 16 g + 15; the next block's pages and scales are asked for before this one's are used.
+    reg_dealloc<TILES_REGS_OTHER>();
+    int64_t left = blockIdx.x;              // items between the walk's place and this block's next item
+    int req = 0;
+    uint32_t blocks = 0;
+    bool ok = true;
+    for (uint32_t k_item = 0; ok; ++k_item) {
+      Request r{0, 0, 0};
+      bool go = false;
+      for (; req < p.B; ++req) {
+        r = request_of(p, req);
+        const int64_t n = request_items(p, r);
+        if (left < n) {
+          go = true;
+          break;
         }
+        left -= n;
       }
-      __syncwarp();
-      blocks += it.nmax;
-      meet();
+      const int pairs = max(1, (r.n * p.G + 2 * TM - 1) / (2 * TM)), idx = static_cast<int>(left);
+      const int head = idx / pairs, row0 = (pairs - 1 - idx % pairs) * 2 * TM;
+      left += gridDim.x;
+      if (!mbar_wait(&sm.item_empty[k_item % ITEMS], ((k_item / ITEMS) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+      if (lane == 0) {
+        sm.item[k_item % ITEMS] = TilesItem{r.t0, r.n, r.len, head, row0, go, {0, 0}};
+        mbar_arrive(&sm.item_full[k_item % ITEMS]);
       }
-    } else if (warp == 9) {
-      // ------------------------------------------------------------------ pages and codes
-      // lane g < 8 looks after the block's keys 16 g .. 16 g + 15; the next block's page and scales are asked for
-      // before this one's ring entries are waited for
-      reg_dealloc<TILES_REGS_OTHER>();
-      if (lane == 0) find_item();
-      Item it;
-      while (begin_item(it)) {
-      const int len = it.len, head = it.head, nmax = it.nmax, req = it.req;
+      // the item's queries on their way to L2
+      for (int R = row0 + lane; go && R < min(row0 + 2 * TM, r.n * p.G); R += 32) {
+        const int token = R / p.G;
+        const T* q = static_cast<const T*>(p.Q) + (r.t0 + token) * p.q_st + (head * p.G + R - token * p.G) * p.q_sh;
+#pragma unroll
+        for (int k = 0; k < D; k += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + k));
+      }
+      const int nmax = go ? max(blocks_of(row0, r.n, r.len), blocks_of(row0 + TM, r.n, r.len)) : 1;
       int pid = -1, row = 0;
       float ks = 0.f, vs = 0.f;
       auto look_up = [&](int j) {
-        const int key = j * TN + 16 * lane;
+        const int key = j * BN + 16 * lane;
         pid = -1;
         ks = vs = 0.f;
-        if (lane < 8 && j < nmax && key < len) {
+        if (go && lane < 8 && j < nmax && key < r.len) {
           const int w = key / p.page;
           row = key - w * p.page;
           pid = p.table[req * p.table_stride + w];
@@ -456,10 +579,11 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       };
       look_up(0);
       int vexp = -1000;
-      bool ok = true;
-      for (int j = 0; j < nmax && ok; ++j) {
+      for (int j = 0; j < nmax; ++j) {
         const uint32_t b = blocks + j;
         const int page = pid, at = row;
+        const float ks_now = ks, vs_now = vs;
+        look_up(j + 1);
         // scale = f 2^e; zero, subnormal, infinite and NaN scales go into f, at the reference's exponent
         auto exponent = [](float s) {
           const int x = static_cast<int>((__float_as_uint(s) >> 23) & 255u);
@@ -470,16 +594,18 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           return s * pow2f(-ref / 2) * pow2f(-ref + ref / 2);
         };
         const bool there = page >= 0;
-        const int ek = there ? exponent(ks) : -1000, ev = there ? exponent(vs) : -1000;
+        const int ek = there ? exponent(ks_now) : -1000, ev = there ? exponent(vs_now) : -1000;
         const int kmax = __reduce_max_sync(0xffffffffu, ek), vmax = __reduce_max_sync(0xffffffffu, ev);
         const int kref = kmax == -1000 ? 0 : kmax, vold = vexp;
         vexp = max(vexp, vmax);
         const int vnow = vexp == -1000 ? 0 : vexp;
-        const float fk = there ? rest(ks, ek, kref) : 1.f, fv = there ? rest(vs, ev, vnow) : 1.f;
+        const float fk = there ? rest(ks_now, ek, kref) : 1.f, fv = there ? rest(vs_now, ev, vnow) : 1.f;
         const uint32_t gone = __ballot_sync(0xffffffffu, page == -2);
-        const bool all_plain = __all_sync(0xffffffffu, page != -2 && fk == 1.f);
-        look_up(j + 1);
-        ok = mbar_wait(&sm.raw_empty[0], (b & 1u) ^ 1u, abort_flag);
+        const bool plain = __all_sync(0xffffffffu, page != -2 && fk == 1.f);
+        const bool whole = gone == 0 && r.len - j * BN >= BN;
+        const bool unit_k = __all_sync(0xffffffffu, !there || ek == kref), unit_v = __all_sync(0xffffffffu, !there || ev == vnow);
+        const bool plain_v = __all_sync(0xffffffffu, fv == 1.f);
+        if (!mbar_wait(&sm.raw_empty[0], (b & 1u) ^ 1u, abort_flag)) { ok = false; break; }
         BlockRecord& rec = sm.rec[b % RECORDS];
         if (lane < 8) {
           rec.rk[lane] = f16x2_pow2(ek == -1000 ? 0 : ek - kref);
@@ -491,105 +617,121 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           rec.kref = pow2f(kref);
           rec.vref = pow2f(vnow);
           rec.vshift = j == 0 || vold == vexp ? 1.f : (vold == -1000 ? pow2f(-vexp) : pow2f(vold - vexp));
-          rec.plain = all_plain;
+          rec.plain = plain;
           rec.gone = gone;
+          rec.mode[0] = !whole ? 2 : (unit_k ? 0 : 1);
+          rec.mode[1] = !whole || !plain_v ? 2 : (unit_v ? 0 : 1);
+          rec.have = go ? min(r.len - j * BN, BN) : -1;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.rec_full[b % RECORDS]);
+        if (!go) break;
+        // (with boxes of 32 rows an even group brings the odd one behind it)
+        const bool issue = there && (p.box == 16 || (lane & 1) == 0);
+        const uint32_t bytes = __reduce_add_sync(0xffffffffu, issue ? p.box * D : 0);
 #pragma unroll
         for (int side = 0; side < 2; ++side) {
-          if (side == 1) ok = ok && mbar_wait(&sm.raw_empty[1], (b & 1u) ^ 1u, abort_flag);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          const bool issue = there && lane < 8 && (p.box == 16 || (lane & 1) == 0);
-          const uint32_t bytes = __reduce_add_sync(0xffffffffu, issue ? p.box * D : 0);
+          if (side == 1 && !mbar_wait(&sm.raw_empty[1], (b & 1u) ^ 1u, abort_flag)) { ok = false; break; }
           if (lane == 0) mbar_expect_tx(&sm.raw_full[side], bytes);
           __syncwarp();
           if (issue) tma_load_4d(sm.raw[side] + lane * 16 * D, side ? &tmV : &tmK, &sm.raw_full[side], 0, at, head, page);
         }
+        if (!ok) break;
       }
-      if (!ok) {
-        give_up();
-        int zero = 0;
-        for (int s = 0; s < 2; ++s) mbar_wait(&sm.raw_full[s], blocks & 1u, &zero, 2000000ull);
-      }
-      __syncwarp();
+      if (!go) break;
       blocks += nmax;
-      meet();                               // (the item's description is not read any more)
-      if (lane == 0) find_item();
+    }
+    if (!ok) {
+      give_up();
+      int zero = 0;                         // let the copies that were issued land before the block goes away
+      for (int s = 0; s < 2; ++s) {
+        mbar_wait(&sm.raw_full[s], 0, &zero, 2000000ull);
+        mbar_wait(&sm.raw_full[s], 1, &zero, 2000000ull);
       }
-    } else if (warp >= 12) {
-      // ------------------------------------------------------------------ codes to f16
-      reg_dealloc<TILES_REGS_OTHER>();
-      Item it;
-      while (begin_item(it)) {
-      const int len = it.len, nmax = it.nmax;
-      const int ct = tid - 384;
-      constexpr int CPR = D / 16;           // 16-code chunks of a row
-      bool ok = true;
-      for (int j = 0; j < nmax && ok; ++j) {
-        const uint32_t b = blocks + j, slot = b & 1u;
-        const BlockRecord& rec = sm.rec[b % RECORDS];
-        const int have = len - j * TN;      // rows behind the last token become zero
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ codes to f16
+    // A thread turns 16-byte pieces into two: of row r0 + STEP x, always the same column.  STEP is a multiple of 8, so
+    // the swizzle is the same in every row it meets and its addresses differ by constants.
+    reg_dealloc<TILES_REGS_OTHER>();
+    constexpr int CPR = D / 16;             // pieces of a row
+    constexpr int STEP = CONVERT_WARPS * 32 / CPR, PIECES = (BN + STEP - 1) / STEP;
+    static_assert(STEP % 8 == 0, "");
+    const int ct = tid - (TILES_THREADS - CONVERT_WARPS * 32), r0 = ct / CPR, ch = ct % CPR;
+    // The two 128-byte lines a row of D = 128 becomes share banks: threads of the second write their halves in the other order.
+    const int swap = D == 128 ? ch >> 2 : 0;
+    const uint32_t src0 = smem_u32(sm.raw[0]) + tile_offset<D>(r0, ch) + swap * 8;
+    const uint32_t dst0 = smem_u32(sm.k[0]) + (ch >> 2) * 16384 + r0 * 128;
+    const uint32_t first = ((2 * (ch & 3) + swap) ^ (r0 & 7)) << 4, second = ((2 * (ch & 3) + 1 - swap) ^ (r0 & 7)) << 4;
+    static_assert(offsetof(Smem, v) - offsetof(Smem, k) == 2 * TILE, "V's tiles stand behind K's");
+    bool ok = true;
+    for (uint32_t b = 0; ok; ++b) {
+      if (!mbar_wait(&sm.rec_full[b % RECORDS], (b / RECORDS) & 1u, abort_flag)) { ok = false; break; }
+      const BlockRecord& rec = sm.rec[b % RECORDS];
+      if (rec.have < 0) break;
+      const uint32_t slot = b & 1u;
+      const int have = rec.have;
+      const uint32_t gone = rec.gone;
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {
-          uint64_t* empty = side ? &sm.v_empty[slot] : &sm.k_empty[slot];
-          if (side == 0) ok = mbar_wait(&sm.rec_full[b % RECORDS], (b / RECORDS) & 1u, abort_flag);
-          ok = ok && mbar_wait(&sm.raw_full[side], b & 1u, abort_flag) && mbar_wait(empty, ((b >> 1) & 1u) ^ 1u, abort_flag);
-          if (!ok) break;
-          const uint8_t* raw = sm.raw[side];
-          uint8_t* tile = side ? sm.v[slot] : sm.k[slot];
-          const uint32_t* ratio = side ? rec.rv : rec.rk;
-          const uint32_t gone = rec.gone;
-#pragma unroll 4
-          for (int it = 0; it < TN * CPR / 128; ++it) {
-            const int idx = it * 128 + ct, r = idx / CPR, ch = idx % CPR;
-            uint32_t w[4], h[8];
-            lds128(smem_u32(raw) + tile_offset<D>(r, ch), w);
-            const uint32_t f = ratio[r >> 4];
-            const bool nothing = r >= have || ((gone >> (r >> 4)) & 1u);
+      for (int side = 0; side < 2; ++side) {
+        if (!mbar_wait(&sm.raw_full[side], b & 1u, abort_flag) ||
+            !mbar_wait(side ? &sm.v_empty[slot] : &sm.k_empty[slot], ((b >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+        const uint32_t src = src0 + side * (BN * D), dst = dst0 + (side * 2 + slot) * TILE;
+        auto convert = [&](auto how) {
+          constexpr int kMode = decltype(how)::value;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              e4m3x4_to_f16(w[x], h[2 * x], h[2 * x + 1]);
-              h[2 * x] = hmul2(h[2 * x], f);
-              h[2 * x + 1] = hmul2(h[2 * x + 1], f);
+          for (int x = 0; x < PIECES; ++x) {
+            const int r = r0 + STEP * x;
+            if (STEP * x + STEP > BN && r >= BN) break;
+            uint32_t w[2][2], h[2][4];
+            lds64(src + x * STEP * D, w[0]);
+            lds64((src + x * STEP * D) ^ 8u, w[1]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) e4m3x4_to_f16(w[e][y], h[e][2 * y], h[e][2 * y + 1]);
+            if constexpr (kMode > 0) {
+              const uint32_t f = (side ? rec.rv : rec.rk)[r >> 4];
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) h[e][y] = hmul2(h[e][y], f);
             }
-            if (side == 1 && rec.fv[r >> 4] != 1.f) {
+            if constexpr (kMode == 2) {
+              const float fv = side ? rec.fv[r >> 4] : 1.f;
+              const bool nothing = r >= have || ((gone >> (r >> 4)) & 1u);   // (the bytes may be anything)
 #pragma unroll
-              for (int x = 0; x < 8; ++x) {
-                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[x]));
-                h[x] = pack_f16(v.x * rec.fv[r >> 4], v.y * rec.fv[r >> 4]);
-              }
-            }
-            if (nothing) {                  // (the bytes may be anything)
+              for (int e = 0; e < 2; ++e)
 #pragma unroll
-              for (int x = 0; x < 8; ++x) h[x] = 0u;
+                for (int y = 0; y < 4; ++y) {
+                  uint32_t v = h[e][y];
+                  if (fv != 1.f) {
+                    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                    v = pack_f16(a.x * fv, a.y * fv);
+                  }
+                  h[e][y] = nothing ? 0u : v;
+                }
             }
-            // chunks 2 c, 2 c + 1 of the row's 128-byte line in block ch / 4; the lines of the two blocks share banks, so
-            // the second block's are written in the other order
-            uint8_t* line = tile + (ch >> 2) * 16384 + r * 128;
-            const int swap = D == 128 ? ch >> 2 : 0, c0 = 2 * (ch & 3) + swap, c1 = 2 * (ch & 3) + 1 - swap;
-            const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
-            *reinterpret_cast<uint4*>(line + ((c0 ^ (r & 7)) << 4)) = swap ? hi : lo;
-            *reinterpret_cast<uint4*>(line + ((c1 ^ (r & 7)) << 4)) = swap ? lo : hi;
+            sts128(dst + x * STEP * 128 + first, h[0]);
+            sts128(dst + x * STEP * 128 + second, h[1]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&sm.raw_empty[side]);
-            mbar_arrive(side ? &sm.v_full[slot] : &sm.k_full[slot]);
-          }
+        };
+        const int mode = rec.mode[side];
+        if (mode == 0) convert(std::integral_constant<int, 0>{});
+        else if (mode == 1) convert(std::integral_constant<int, 1>{});
+        else convert(std::integral_constant<int, 2>{});
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&sm.raw_empty[side]);
+          mbar_arrive(side ? &sm.v_full[slot] : &sm.k_full[slot]);
         }
       }
-      if (!ok) give_up();
-      __syncwarp();
-      blocks += it.nmax;
-      meet();
-      }
-    } else {
-      reg_dealloc<TILES_REGS_OTHER>();      // warps 10, 11
-      Item it;
-      while (begin_item(it)) meet();
     }
+    if (!ok) give_up();
+  }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {
@@ -604,6 +746,6 @@ int launch_tiles(const CachedParams& p, const CUtensorMap& tmK, const CUtensorMa
   static_assert(SMEM <= 227 * 1024, "a block does not fit an SM's shared memory");
   auto kern = cached_tiles_kernel<T, D>;
   KCG_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-  kern<<<sm_count(), TILES_THREADS, SMEM, stream>>>(tmK, tmV, p, make_idesc(0, 0, 0, 0, TM, TN), make_idesc(0, 0, 0, 1, TM, D));
+  kern<<<sm_count(), TILES_THREADS, SMEM, stream>>>(tmK, tmV, p, make_idesc(0, 0, 0, 0, TM, BN), make_idesc(0, 0, 0, 1, TM, D));
   return check_launch("cached_tiles_kernel");
 }
