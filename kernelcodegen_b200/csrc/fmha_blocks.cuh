@@ -94,7 +94,10 @@ struct NoHook {
 // decided() is called (by all lanes) as soon as this block's value of m is final — before the
 // exponentials on the ordinary path — and wait_o() before the accumulator is touched for a rescale
 // (it returns false if its wait timed out; the rescale is then skipped and the caller gives up).
-template <typename T, int D, typename Arrive, typename Decided = NoHook, typename WaitO = NoHook>
+// kEmuMask: which pairs of exponentials take the FMA pipe (0 where a NaN score must stay one); kThreshold: the growth of
+// the maximum, in log2 units, that O is not rescaled for.
+template <typename T, int D, int kEmuMask = KCG_FMHA_EMU_MASK, int kThreshold = static_cast<int>(kRescaleThreshold), typename Arrive,
+          typename Decided = NoHook, typename WaitO = NoHook>
 __device__ __forceinline__ bool softmax_block(uint32_t s_addr, uint32_t o_addr, int j, int limit, float c, float& m,
                                               float& l, int lane, Arrive arrive, Decided decided = Decided(),
                                               WaitO wait_o = WaitO()) {
@@ -127,7 +130,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_addr, uint32_t o_addr, 
     for (int k = half * 64; k < half * 64 + 64; k += 2) {
       const uint64_t x2 = f2_fma(f2_pack(__uint_as_float(sreg[k]), __uint_as_float(sreg[k + 1])), c2, nm2);
       float p0, p1;
-      if (KCG_FMHA_EMU_MASK != 0 && ((k >> 1) & KCG_FMHA_EMU_MASK) == KCG_FMHA_EMU_MASK) {
+      if (kEmuMask != 0 && ((k >> 1) & kEmuMask) == kEmuMask) {
         exp2_pair_fma(x2, p0, p1);
       } else {
         float x0, x1;
@@ -159,7 +162,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_addr, uint32_t o_addr, 
   if (speculate) {
     const float neg_m0 = -m;
     exp_half(0, f2_pack(neg_m0, neg_m0));
-    if (!__any_sync(0xffffffffu, mt > m + kRescaleThreshold)) {
+    if (!__any_sync(0xffffffffu, mt > m + static_cast<float>(kThreshold))) {
       decided();
       hand_over(0);
       half0_done = true;
@@ -172,7 +175,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_addr, uint32_t o_addr, 
   }
   if (!half0_done) {
     bool rescale = false;
-    if ((mt > m + kRescaleThreshold || m == -INFINITY) && mt > m) {
+    if ((mt > m + static_cast<float>(kThreshold) || m == -INFINITY) && mt > m) {
       alpha = (m == -INFINITY) ? 0.f : fast_exp2(m - mt);
       rescale = (j > 0);
       m = mt;

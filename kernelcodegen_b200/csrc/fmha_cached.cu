@@ -26,6 +26,7 @@
 #include "common.cuh"
 #include "tcgen05.cuh"
 
+#include <atomic>
 #include <cstddef>
 #include <type_traits>
 
@@ -990,6 +991,17 @@ __global__ void __launch_bounds__(JWARPS * 32) cached_join_kernel(const CachedPa
   }
 }
 
+// Kernel attributes are set once per device: `done` is a bit per device of one kernel.
+int once_per_device(std::atomic<uint64_t>& done, cudaError_t (*set)()) {
+  int dev = 0;
+  KCG_CUDA_OK(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_relaxed) & bit)) return KCG_OK;
+  KCG_CUDA_OK(set());
+  if (dev < 64) done.fetch_or(bit, std::memory_order_relaxed);
+  return KCG_OK;
+}
+
 // Workspace of the split kernel with 8 NQ rows: two parts per team and head of a group, each the lanes' output registers
 // and (m, l) of every row, and eight ints per team.
 size_t split_workspace(int64_t D, int nq, int teams) {
@@ -1017,13 +1029,20 @@ int launch_split(CachedParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV
   constexpr int SMEM = sizeof(SplitSmem<D, NQ>) + 1024;
   static_assert(SMEM <= 227 * 1024, "a block does not fit an SM's shared memory");
   auto kern = cached_split_kernel<T, D, NQ>;
-  KCG_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-  kern<<<blocks, split_threads<NQ>(), SMEM, stream>>>(tmK, tmV, p);
-  int rc = check_launch("cached_split_kernel");
+  static std::atomic<uint64_t> done{0};
+  // (the join may become resident early, so it asks for the split kernel's division of L1 and shared memory)
+  int rc = once_per_device(done, []() {
+    const cudaError_t e = cudaFuncSetAttribute(cached_split_kernel<T, D, NQ>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(cached_join_kernel<T, D, NQ>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  });
   if (rc) return rc;
   if (teams > MAX_TEAMS) return fail(KCG_ERR_UNSUPPORTED, "fmha_cached: a device of %d SMs", blocks);
-  // (the join may become resident early, so it asks for the split kernel's division of L1 and shared memory)
-  KCG_CUDA_OK(cudaFuncSetAttribute(cached_join_kernel<T, D, NQ>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  // Not as a programmatic dependent: a block that becomes resident beside the previous kernel's keeps its SM at that
+  // kernel's split of L1 and shared memory, where this one does not fit, and queues behind it (142 instead of 100 us for
+  // 64 requests of 4096 tokens).
+  kern<<<blocks, split_threads<NQ>(), SMEM, stream>>>(tmK, tmV, p);
+  rc = check_launch("cached_split_kernel");
+  if (rc) return rc;
   launch_overlapped(cached_join_kernel<T, D, NQ>, dim3(2 * blocks), dim3(JWARPS * 32), 0, stream, p, teams);
   return check_launch("cached_join_kernel");
 }

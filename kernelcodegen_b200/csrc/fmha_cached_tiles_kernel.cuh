@@ -24,7 +24,7 @@
 
 constexpr int TM = 128;                 // rows of a tile; BN keys of a block
 constexpr int TILES_THREADS = 512, CONVERT_WARPS = 6;
-constexpr int TILES_REGS_SOFTMAX = 184, TILES_REGS_OTHER = 72;
+constexpr int TILES_REGS_SOFTMAX = 200, TILES_REGS_OTHER = 56;
 static_assert(2 * 128 * (TILES_REGS_SOFTMAX + TILES_REGS_OTHER) <= TILES_THREADS * 128, "register split exceeds the block's allocation");
 // A record is written when the codes of the K tile before it have been converted, which is at most two blocks (the ring of f16
 // tiles) before the softmax is through with that block: it is read at most four blocks after it is written.
@@ -92,104 +92,6 @@ __device__ __forceinline__ bool pv4_peek2(uint32_t d_o, uint32_t a_p, uint64_t v
       : "memory");
   ok2 = r2 != 0;
   return r1 != 0;
-}
-
-// The online softmax of one key block for the calling thread's row, as softmax_block does it, but holding 64 scores at a time:
-// with half of the warps converting, 128 scores and their helpers (about 210 registers) do not fit the softmax warps.
-// Scores are read again from tensor memory where both halves are needed twice.
-template <int D, typename Arrive>
-__device__ __forceinline__ void softmax_halves(uint32_t s_addr, uint32_t o_addr, int j, int limit, float c, float& m, float& l, int lane,
-                                               Arrive arrive) {
-  const uint64_t c2 = f2_pack(c, c);
-  uint64_t sum_a = 0ull, sum_b = 0ull;
-  uint32_t s[64], pk[32];
-  auto load = [&](int half) {
-    tmem_ld64(s_addr + 64 * half, s);
-    tmem_wait_ld();
-    if (limit < BN) {
-#pragma unroll
-      for (int k = 0; k < 64; ++k)
-        if (64 * half + k >= limit) s[k] = 0xff800000u;
-    }
-  };
-  auto maximum = [&]() {
-    float mx[4];
-#pragma unroll
-    for (int a = 0; a < 4; ++a) mx[a] = fmaxf(__uint_as_float(s[2 * a]), __uint_as_float(s[2 * a + 1]));
-#pragma unroll
-    for (int k = 8; k < 64; k += 8)
-#pragma unroll
-      for (int a = 0; a < 4; ++a) mx[a] = max3(mx[a], __uint_as_float(s[k + 2 * a]), __uint_as_float(s[k + 2 * a + 1]));
-    return fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]);
-  };
-  auto exponentials = [&](float base) {
-    const uint64_t nb2 = f2_pack(-base, -base);
-#pragma unroll
-    for (int k = 0; k < 64; k += 2) {
-      float x0, x1;
-      f2_unpack(f2_fma(f2_pack(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c2, nb2), x0, x1);
-      const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-      if ((k >> 1) & 1) sum_b = f2_add(sum_b, f2_pack(p0, p1));
-      else sum_a = f2_add(sum_a, f2_pack(p0, p1));
-      pk[k >> 1] = pack2<__half>(p0, p1);
-    }
-  };
-  auto hand_over = [&](int half) {
-    tmem_st32(s_addr + half * 32, pk);
-    tmem_wait_st();
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) arrive(half);
-  };
-  float alpha = 1.f;
-  bool done = false;
-  // Speculation, as in softmax_block: the first half's exponentials with the maximum so far, before this block's is known.
-  if (__all_sync(0xffffffffu, j > 0 && limit >= BN && m != -INFINITY)) {
-    load(0);
-    exponentials(m);
-    float mt = maximum();
-    load(1);
-    mt = fmaxf(mt, maximum()) * c;
-    if (!__any_sync(0xffffffffu, mt > m + kLazy)) {
-      hand_over(0);
-      exponentials(m);
-      hand_over(1);
-      done = true;
-    } else {
-      sum_a = sum_b = 0ull;
-    }
-  }
-  if (!done) {
-    load(0);
-    float mt = maximum();
-    load(1);
-    mt = fmaxf(mt, maximum()) * c;
-    if (mt > m + kLazy) {
-      alpha = fast_exp2(m - mt);            // 0 for the row's first keys
-      m = mt;
-    }
-    if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-#pragma unroll 1
-      for (int cc = 0; cc < D / 32; ++cc) {
-        tmem_ld32(o_addr + cc * 32, pk);
-        tmem_wait_ld();
-#pragma unroll
-        for (int k = 0; k < 32; ++k) pk[k] = __float_as_uint(__uint_as_float(pk[k]) * alpha);
-        tmem_st32(o_addr + cc * 32, pk);
-        tmem_wait_st();                     // (the registers of a store are not touched before it is done)
-      }
-    }
-    const float base = m == -INFINITY ? 0.f : m;
-    load(0);
-    exponentials(base);
-    hand_over(0);
-    load(1);
-    exponentials(base);
-    hand_over(1);
-  }
-  float l0, l1;
-  f2_unpack(f2_add(sum_a, sum_b), l0, l1);
-  l = l * alpha + (l0 + l1);
 }
 
 __device__ __forceinline__ int64_t request_items(const CachedParams& p, const Request& r) {
@@ -388,7 +290,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             tmem_wait_st();
           }
         }
-        softmax_halves<D>(s_addr, o_addr, j, seen - j * BN, cj, m, l, lane, [&](int half) { mbar_arrive(&sm.p_full[2 * i + half]); });
+        softmax_block<__half, D, 0, static_cast<int>(kLazy)>(s_addr, o_addr, j, seen - j * BN, cj, m, l, lane, [&](int half) { mbar_arrive(&sm.p_full[2 * i + half]); });
       }
       // The next item's scores may be computed while this one's output leaves.
       if (ok && have_q) c = convert_q();
@@ -745,7 +647,9 @@ int launch_tiles(const CachedParams& p, const CUtensorMap& tmK, const CUtensorMa
   constexpr int SMEM = sizeof(TilesSmem<D>) + 1024;
   static_assert(SMEM <= 227 * 1024, "a block does not fit an SM's shared memory");
   auto kern = cached_tiles_kernel<T, D>;
-  KCG_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+  static std::atomic<uint64_t> done{0};
+  const int rc = once_per_device(done, []() { return cudaFuncSetAttribute(cached_tiles_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
+  if (rc) return rc;
   kern<<<sm_count(), TILES_THREADS, SMEM, stream>>>(tmK, tmV, p, make_idesc(0, 0, 0, 0, TM, BN), make_idesc(0, 0, 0, 1, TM, D));
   return check_launch("cached_tiles_kernel");
 }

@@ -13,6 +13,7 @@ kernels, and there is no fallback path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -374,20 +375,8 @@ def fmha(Q, K, V, softmax_scale: float = 1.0, causal: bool = False, out_layout: 
 _workspace_bytes: dict = {}
 
 
-class _On:
-    """Makes a tensor's device current for a launch, when it is not the current one already."""
-    __slots__ = ("guard",)
-
-    def __init__(self, t):
-        self.guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+# The current stream's handle without the Python object around it, which costs as much as the rest of a small call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _vector(what: str, name: str, t, dtype, n=None) -> None:
@@ -395,13 +384,18 @@ def _vector(what: str, name: str, t, dtype, n=None) -> None:
         raise ValueError(f"{what}: {name} must be a contiguous {dtype} vector" + ("" if n is None else f" of {n}"))
 
 
+@functools.lru_cache(maxsize=1024)
+def _outer(shape, stride):
+    return _i64arr([s if n > 1 else 0 for n, s in zip(shape[:-1], stride)])
+
+
 def _outer_strides(t):
     """Strides of all dims but the last; of a dim with one entry (or none) any stride will do: 0."""
-    return _i64arr([s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride())])
+    return _outer(t.shape, t.stride())
 
 
 def _no_overlap(what: str, name: str, t) -> None:
-    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+    if 0 in t.stride() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
         raise ValueError(f"{what}: {name} is written and must not be an expanded view")
 
 
@@ -423,12 +417,15 @@ def _check_cache(what: str, k_cache, v_cache, k_scale, v_scale) -> None:
             raise ValueError(f"{what}: {name} must be a contiguous float32 [pages, Hkv]")
 
 
-def _one_device(what: str, first, *ts) -> None:
+def _one_device(what: str, first, *ts) -> int:
+    """Index of the device all operands are on."""
     if not first.is_cuda:
         raise ValueError("operands must be CUDA tensors (there is no CPU path)")
+    index = first.get_device()
     for t in ts:
-        if t.device != first.device:
+        if t.get_device() != index:
             raise ValueError(f"{what}: operands are on {first.device} and {t.device}")
+    return index
 
 
 def cache_plan(cached, new, block_table, free_pages, free_count, page_size: int, max_tokens: int, out=None):
@@ -452,13 +449,13 @@ def cache_plan(cached, new, block_table, free_pages, free_count, page_size: int,
     _vector(what, "free_count", free_count, torch.int32, 1)
     if max_tokens < 0 or page_size < 1:
         raise ValueError("cache_plan: max_tokens and page_size must not be negative or zero")
-    _one_device(what, cached, new, block_table, free_pages, free_count)
+    index = _one_device(what, cached, new, block_table, free_pages, free_count)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return cache_plan(cached, new, block_table, free_pages, free_count, page_size, max_tokens, out)
     if out is None:
-        dev = cached.device
-        lengths = torch.empty(B, dtype=torch.int32, device=dev)
-        cu_new = torch.empty(B + 1, dtype=torch.int32, device=dev)
-        slot_map = torch.empty(max_tokens, dtype=torch.int64, device=dev)
-        free_left = torch.empty(1, dtype=torch.int32, device=dev)
+        lengths, cu_new, free_left = cached.new_empty(B), cached.new_empty(B + 1), cached.new_empty(1)
+        slot_map = cached.new_empty(max_tokens, dtype=torch.int64)
     else:
         lengths, cu_new, slot_map, free_left = out
         _vector(what, "out lengths", lengths, torch.int32, B)
@@ -466,13 +463,11 @@ def cache_plan(cached, new, block_table, free_pages, free_count, page_size: int,
         _vector(what, "out slot_map", slot_map, torch.int64, max_tokens)
         _vector(what, "out free_left", free_left, torch.int32, 1)
         _one_device(what, cached, lengths, cu_new, slot_map, free_left)
-    with _On(cached):
-        check(_lib.load().kcg_cache_plan(B, page_size, max_tokens, cached.data_ptr(), new.data_ptr(),
-                                         block_table.data_ptr(), block_table.shape[1],
-                                         max(block_table.stride(0), block_table.shape[1]), free_pages.data_ptr(),
-                                         free_pages.shape[0], free_count.data_ptr(), lengths.data_ptr(),
-                                         cu_new.data_ptr(), slot_map.data_ptr(), free_left.data_ptr(), _stream()),
-              "kcg_cache_plan")
+    check(_lib.load().kcg_cache_plan(B, page_size, max_tokens, cached.data_ptr(), new.data_ptr(), block_table.data_ptr(),
+                                     block_table.shape[1], max(block_table.stride(0), block_table.shape[1]),
+                                     free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), lengths.data_ptr(),
+                                     cu_new.data_ptr(), slot_map.data_ptr(), free_left.data_ptr(), _raw_stream(index)),
+          "kcg_cache_plan")
     return lengths, cu_new, slot_map, free_left
 
 
@@ -492,13 +487,14 @@ def cache_append(K, V, slot_map, k_cache, v_cache, k_scale, v_scale) -> None:
     _no_overlap(what, "k_cache", k_cache)
     _no_overlap(what, "v_cache", v_cache)
     _vector(what, "slot_map", slot_map, torch.int64, K.shape[0])
-    _one_device(what, K, V, slot_map, k_cache, v_cache, k_scale, v_scale)
-    with _On(K):
-        check(_lib.load().kcg_cache_append(_dt(K), K.shape[0], Hkv, D, K.data_ptr(), _outer_strides(K), V.data_ptr(),
-                                           _outer_strides(V), slot_map.data_ptr(), pages, page_size,
-                                           k_cache.data_ptr(), _outer_strides(k_cache), v_cache.data_ptr(),
-                                           _outer_strides(v_cache), k_scale.data_ptr(), v_scale.data_ptr(),
-                                           _stream()), "kcg_cache_append")
+    index = _one_device(what, K, V, slot_map, k_cache, v_cache, k_scale, v_scale)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return cache_append(K, V, slot_map, k_cache, v_cache, k_scale, v_scale)
+    check(_lib.load().kcg_cache_append(_dt(K), K.shape[0], Hkv, D, K.data_ptr(), _outer_strides(K), V.data_ptr(),
+                                       _outer_strides(V), slot_map.data_ptr(), pages, page_size, k_cache.data_ptr(),
+                                       _outer_strides(k_cache), v_cache.data_ptr(), _outer_strides(v_cache),
+                                       k_scale.data_ptr(), v_scale.data_ptr(), _raw_stream(index)), "kcg_cache_append")
 
 
 def fmha_cached(Q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, cu_new=None, softmax_scale: float = 1.0,
@@ -526,29 +522,29 @@ def fmha_cached(Q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, cu_
         _vector(what, "cu_new", cu_new, torch.int32, B + 1)
     elif B == 0 or T % B:
         raise ValueError(f"{what}: without cu_new, {T} rows must divide into {B} requests")
-    _one_device(what, Q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, *(() if cu_new is None else (cu_new,)))
+    index = _one_device(what, Q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, lengths if cu_new is None else cu_new)
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return fmha_cached(Q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, cu_new, softmax_scale, causal,
+                               max_new, out)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=Q.dtype, device=Q.device)
+        out = Q.new_empty((T, Hq, D))
     elif out.shape != Q.shape or out.dtype != Q.dtype or out.device != Q.device or out.stride(2) != 1:
         raise ValueError(f"{what}: out must be a {tuple(Q.shape)} {Q.dtype} tensor on {Q.device} with a contiguous last dim")
     else:
         _no_overlap(what, "out", out)
-    with _On(Q):
-        lib = _lib.load()
-        key = (Q.device.index, D)
-        nbytes = _workspace_bytes.get(key)
-        if nbytes is None:
-            size = ctypes.c_size_t()
-            check(lib.kcg_fmha_cached_workspace(D, ctypes.byref(size)), "kcg_fmha_cached_workspace")
-            nbytes = _workspace_bytes[key] = size.value
-        # from the caching allocator, on the launching stream: calls on other streams get memory of their own
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=Q.device)
-        check(lib.kcg_fmha_cached_fwd(_dt(Q), T, B, Hq, Hkv, D, max_new, float(softmax_scale), int(causal), Q.data_ptr(),
-                                      _outer_strides(Q), k_cache.data_ptr(), _outer_strides(k_cache),
-                                      k_scale.data_ptr(), v_cache.data_ptr(), _outer_strides(v_cache),
-                                      v_scale.data_ptr(), pages, page_size, block_table.data_ptr(), block_table.shape[1],
-                                      max(block_table.stride(0), block_table.shape[1]), lengths.data_ptr(),
-                                      None if cu_new is None else cu_new.data_ptr(), out.data_ptr(),
-                                      _outer_strides(out), workspace.data_ptr(), nbytes, _stream()),
-              "kcg_fmha_cached_fwd")
+    lib = _lib.load()
+    nbytes = _workspace_bytes.get((index, D))
+    if nbytes is None:
+        size = ctypes.c_size_t()
+        check(lib.kcg_fmha_cached_workspace(D, ctypes.byref(size)), "kcg_fmha_cached_workspace")
+        nbytes = _workspace_bytes[index, D] = size.value
+    # from the caching allocator, on the launching stream: calls on other streams get memory of their own
+    workspace = lengths.new_empty(nbytes, dtype=torch.uint8)
+    check(lib.kcg_fmha_cached_fwd(_dt(Q), T, B, Hq, Hkv, D, max_new, softmax_scale, causal, Q.data_ptr(), _outer_strides(Q),
+                                  k_cache.data_ptr(), _outer_strides(k_cache), k_scale.data_ptr(), v_cache.data_ptr(),
+                                  _outer_strides(v_cache), v_scale.data_ptr(), pages, page_size, block_table.data_ptr(),
+                                  block_table.shape[1], max(block_table.stride(0), block_table.shape[1]), lengths.data_ptr(),
+                                  None if cu_new is None else cu_new.data_ptr(), out.data_ptr(), _outer_strides(out),
+                                  workspace.data_ptr(), nbytes, _raw_stream(index)), "kcg_fmha_cached_fwd")
     return out
