@@ -888,17 +888,9 @@ cached_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 // reads the items of all teams, then a warp asks for EARLY parts and their maxima and sums at once.  The order of the
 // sums depends on sizes alone.
 constexpr int JWARPS = 8, EARLY = 8, MAX_TEAMS = 1024;
-template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(JWARPS * 32) cached_join_kernel(const CachedParams p, int teams) {
-  constexpr int MT = D / 16, ROWS = 8 * NQ, NREG = NQ * MT * 4;
-  __shared__ float s_acc[JWARPS][8][32];
-  __shared__ uint16_t s_team[MAX_TEAMS];              // teams whose last item goes on behind them
-  __shared__ int s_count[JWARPS];
-  grid_launch_dependents();
-  grid_dependency_wait();
+// Lists the teams whose last item goes on behind them (their first meta word is set); called by a block of JWARPS warps.
+__device__ __forceinline__ int open_items(const CachedParams& p, int teams, uint16_t* s_team, int* s_count) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  const int4* meta = reinterpret_cast<const int4*>(p.meta);   // set, last team, slot, t0; n, head, rb
   int items = 0;
   for (int c0 = 0; c0 < teams; c0 += JWARPS * 32) {
     const int c = c0 + threadIdx.x;
@@ -915,6 +907,20 @@ __global__ void __launch_bounds__(JWARPS * 32) cached_join_kernel(const CachedPa
     if (open) s_team[before + __popc(mask & ((1u << lane) - 1))] = static_cast<uint16_t>(c);
     __syncthreads();
   }
+  return items;
+}
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(JWARPS * 32) cached_join_kernel(const CachedParams p, int teams) {
+  constexpr int MT = D / 16, ROWS = 8 * NQ, NREG = NQ * MT * 4;
+  __shared__ float s_acc[JWARPS][8][32];
+  __shared__ uint16_t s_team[MAX_TEAMS];              // teams whose last item goes on behind them
+  __shared__ int s_count[JWARPS];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int4* meta = reinterpret_cast<const int4*>(p.meta);   // set, last team, slot, t0; n, head, rb
+  const int items = open_items(p, teams, s_team, s_count);
   const int heads = WARPS >> p.wk_log2, tiles = heads * NQ * MT, jobs = items * tiles;
   int split = static_cast<int>(gridDim.x) * JWARPS / max(jobs, 1);
   split = split >= 8 ? 8 : (split >= 4 ? 4 : (split >= 2 ? 2 : 1));
@@ -1055,7 +1061,7 @@ int launch_cached(CachedParams& p, int64_t rows, const CUtensorMap& tmK, const C
   // Two heads side by side where there are two: as fast as four or one with a head's page in one piece, and 20 % faster
   // than one where a token's heads stand together (8 x 4096 tokens of 32 heads, token-major: 54.8 us, one head 68.2).
   p.wk_log2 = p.Hkv % 2 == 0 ? 1 : 2;
-  if (rows > 16) return launch_tiles<T, D>(p, tmK, tmV, stream);
+  if (rows > 16) return launch_tiles<T, D>(p, tmK, tmV, workspace, stream);
   if (rows <= 8) return launch_split<T, D, 1>(p, tmK, tmV, items, workspace, stream);
   return launch_split<T, D, 2>(p, tmK, tmV, items * ((rows + 15) / 16), workspace, stream);
 }
@@ -1069,7 +1075,9 @@ extern "C" int kcg_fmha_cached_workspace(int64_t D, size_t* bytes) {
   if (!bytes) return fail(KCG_ERR_INVALID_ARG, "fmha_cached_workspace: null pointer");
   if (D != 64 && D != 128) return fail(KCG_ERR_UNSUPPORTED, "fmha_cached: head dimension %lld has no kernel (64, 128)", static_cast<long long>(D));
   const size_t one = split_workspace(D, 1, split_teams(1)), two = split_workspace(D, 2, split_teams(2));
+  const size_t many = tiles_workspace(D, sm_count());
   *bytes = one > two ? one : two;
+  if (many > *bytes) *bytes = many;
   return KCG_OK;
 }
 

@@ -3,13 +3,16 @@
 // two-tile kernel of fmha_tcgen05.cu:
 //
 //   An item is a pair of 128-row tiles of one (request, key / value head): rows are (token, query head of the group) in
-//   token-major order, so a block of 128 keys is loaded and converted once for 256 rows, whatever the group.
+//   token-major order, so a block of 128 keys is loaded and converted once for 256 rows, whatever the group.  The key
+//   blocks of all items, numbered by request, head, pair and keys, are dealt to the SMs in equal contiguous ranges, as the
+//   split kernel deals its units: prompts of any lengths end together, and a short chunk against a long context is
+//   spread over all SMs.  A range's first and last item may be parts, which cached_tiles_join_kernel merges.
 //   warps 0-3, 4-7  softmax of tile 0 / 1, one thread per row (scores, P and O in tensor memory); before that, the row
 //                   of Q, as f16 scaled by a power of two, into the swizzled tile the products read; afterwards, O out
 //   warp 8          one thread issues the products: S_i = Q_i K^T, O_i += P_i V, S_i(j + 1) right behind P_i V(j)
 //   warp 9          walks the items, looks pages and scales up (a record per key block) and loads the codes of K and V by
 //                   TMA (boxes of 16 or 32 rows of a page)
-//   warps 10-15     turn codes into f16 tiles in the swizzled layout tcgen05 wants, the same for K and V
+//   warps 10, 11    turn codes into f16 tiles in the swizzled layout tcgen05 wants, the same for K and V
 // Every ring and barrier runs on across items: records, codes and the first tiles of the next item are on their way while
 // the last blocks of this one are worked on.
 //
@@ -23,9 +26,9 @@
 #pragma once
 
 constexpr int TM = 128;                 // rows of a tile; BN keys of a block
-constexpr int TILES_THREADS = 512, CONVERT_WARPS = 6;
-constexpr int TILES_REGS_SOFTMAX = 200, TILES_REGS_OTHER = 56;
-static_assert(2 * 128 * (TILES_REGS_SOFTMAX + TILES_REGS_OTHER) <= TILES_THREADS * 128, "register split exceeds the block's allocation");
+constexpr int TILES_THREADS = 384, CONVERT_WARPS = 2;
+constexpr int TILES_REGS_SOFTMAX = 216, TILES_REGS_OTHER = 72;
+static_assert(256 * TILES_REGS_SOFTMAX + (TILES_THREADS - 256) * TILES_REGS_OTHER <= TILES_THREADS * 168, "register split exceeds the block's allocation");
 // A record is written when the codes of the K tile before it have been converted, which is at most two blocks (the ring of f16
 // tiles) before the softmax is through with that block: it is read at most four blocks after it is written.
 constexpr int RECORDS = 6, ITEMS = 4;
@@ -43,8 +46,11 @@ struct BlockRecord {
   float fk[8], fv[8];                   // f
 };
 struct TilesItem {
-  int t0, n, len, head, row0, go;       // the request's first row of Q, rows, keys; key head; first row of the pair
-  int pad[2];
+  int t0, n, len, head, row0;           // the request's first row of Q, rows, keys; key head; first row of the pair
+  int go;                               // 0: there is no item and none will come
+  int block0, blocks;                   // the part: its first key block, and how many it has
+  int part;                             // where the result goes: -1: O, else the workspace's part
+  int pad[3];
 };
 
 template <int D> struct TilesSmem {
@@ -56,6 +62,8 @@ template <int D> struct TilesSmem {
   TilesItem item[ITEMS];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], rec_full[RECORDS], raw_full[2], raw_empty[2], item_full[ITEMS], item_empty[ITEMS];
   uint64_t q_full, s_full[2], p_full[4], o_full[2], drain;
+  int64_t scan[16], start_off;
+  int start_i;
   uint32_t tmem;
   int abort;
 };
@@ -94,8 +102,25 @@ __device__ __forceinline__ bool pv4_peek2(uint32_t d_o, uint32_t a_p, uint64_t v
   return r1 != 0;
 }
 
-__device__ __forceinline__ int64_t request_items(const CachedParams& p, const Request& r) {
-  return static_cast<int64_t>(p.Hkv) * ((r.n * p.G + 2 * TM - 1) / (2 * TM));
+// Key blocks of the tile of rows that begins at `first`: up to the last key its last row sees.
+__device__ __forceinline__ int tile_blocks(const CachedParams& p, int first, int n, int len) {
+  const int last = min(first + TM, n * p.G) - 1;
+  if (last < first) return 0;
+  const int end = p.causal ? min(len, len - n + 1 + last / p.G) : len;
+  return end > 0 ? (end + BN - 1) / BN : 0;
+}
+__device__ __forceinline__ int pair_blocks(const CachedParams& p, int row0, int n, int len) {
+  return max(tile_blocks(p, row0, n, len), tile_blocks(p, row0 + TM, n, len));
+}
+__device__ __forceinline__ int pairs_of(const CachedParams& p, const Request& r) { return (r.n * p.G + 2 * TM - 1) / (2 * TM); }
+// Units of one head of a request; a pair that sees nothing still has to write its zeros.
+__device__ __forceinline__ int64_t head_units(const CachedParams& p, const Request& r) {
+  const int pairs = pairs_of(p, r);
+  if (pairs == 0) return 0;
+  if (!p.causal) return static_cast<int64_t>(pairs) * max(1, pair_blocks(p, 0, r.n, r.len));
+  int64_t units = 0;
+  for (int k = 0; k < pairs; ++k) units += max(1, pair_blocks(p, k * 2 * TM, r.n, r.len));
+  return units;
 }
 
 template <typename T, int D>
@@ -147,12 +172,49 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       if (p.status) *p.status = KCG_ERR_TIMEOUT;
     }
   };
-  // key blocks of the tile of rows that begins at `first`: up to the last key its last row sees
-  auto blocks_of = [&](int first, int n, int len) {
-    const int last = min(first + TM, n * p.G) - 1;
-    if (last < first) return 0;
-    const int end = p.causal ? min(len, len - n + 1 + last / p.G) : len;
-    return end > 0 ? (end + BN - 1) / BN : 0;
+  // ---- this block's range of units ----
+  const int per = (p.B + TILES_THREADS - 1) / TILES_THREADS;
+  const int i_lo = min(tid * per, p.B), i_hi = min(i_lo + per, p.B);
+  int64_t total = 0, first_unit = 0;
+  int units = 0;
+  {
+    int64_t mine = 0;
+    for (int i = i_lo; i < i_hi; ++i) mine += p.Hkv * head_units(p, request_of(p, i));
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t u = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += u;
+    }
+    if (lane == 31) sm.scan[warp] = upto;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TILES_THREADS / 32; ++w) {
+      if (w < warp) upto += sm.scan[w];
+      total += sm.scan[w];
+    }
+    const int64_t grid = min(static_cast<int64_t>(gridDim.x), total);   // blocks at work
+    if (blockIdx.x < grid) {
+      first_unit = total * blockIdx.x / grid;
+      units = static_cast<int>(total * (blockIdx.x + 1) / grid - first_unit);
+    }
+    int64_t off = first_unit - (upto - mine);
+    if (units > 0 && off >= 0 && off < mine) {           // one thread's requests hold the first unit
+      int i = i_lo;
+      for (;; ++i) {
+        const int64_t n = p.Hkv * head_units(p, request_of(p, i));
+        if (off < n) break;
+        off -= n;
+      }
+      sm.start_i = i;
+      sm.start_off = off;
+    }
+    if (tid == 0) p.meta[blockIdx.x * 8] = -1;
+    __syncthreads();
+  }
+  // blocks of tile i in an item's part
+  auto blocks_of = [&](int i, const TilesItem& it) {
+    return min(max(tile_blocks(p, it.row0 + i * TM, it.n, it.len) - it.block0, 0), it.blocks);
   };
 
   if (warp < 8) {
@@ -231,11 +293,11 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const TilesItem& it = sm.item[k_item % ITEMS];
       if (!it.go) break;
       // key blocks of this tile and of the other; keys this row sees from block b on
-      const int n_mine = blocks_of(it.row0 + i * TM, it.n, it.len), n_other = blocks_of(it.row0 + (1 - i) * TM, it.n, it.len);
+      const int n_mine = blocks_of(i, it), n_other = blocks_of(1 - i, it);
       int seen = 0;
       {
         const int R = it.row0 + i * TM + r;
-        if (R < it.n * p.G) seen = p.causal ? min(it.len, it.len - it.n + 1 + R / p.G) : it.len;
+        if (R < it.n * p.G) seen = (p.causal ? min(it.len, it.len - it.n + 1 + R / p.G) : it.len) - it.block0 * BN;
       }
       if (!have_q) {
         fetch_q(it);
@@ -301,14 +363,26 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       }
       if (!ok) break;
       {
-        const float inv = l == 0.f ? 0.f : vref / l;     // a row that sees no key is zero
-        const int64_t at = offset_of(it, p.o_st, p.o_sh);
+        const int part = it.part;
+        // a row that sees no key is zero; a part keeps its sums as they are
+        const float inv = l == 0.f ? 0.f : (part < 0 ? vref / l : vref);
+        const int64_t at = part < 0 ? offset_of(it, p.o_st, p.o_sh) : 0;
+        float* po = p.part_o + (static_cast<int64_t>(part) * 2 * TM + i * TM + r) * D;
+        if (part >= 0) *reinterpret_cast<float2*>(p.part_ml + (static_cast<int64_t>(part) * 2 * TM + i * TM + r) * 2) = make_float2(m, l);
 #pragma unroll 1
         for (int cc = 0; cc < D / 32; ++cc) {
           uint32_t x[32];
           if (n_mine > 0) {
             tmem_ld32(o_addr + cc * 32, x);
             tmem_wait_ld();
+          }
+          if (part >= 0) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) x[k] = l == 0.f ? 0u : __float_as_uint(__uint_as_float(x[k]) * inv);
+#pragma unroll
+            for (int k = 0; k < 32; k += 8)
+              st_256(po + cc * 32 + k, make_uint4(x[k], x[k + 1], x[k + 2], x[k + 3]), make_uint4(x[k + 4], x[k + 5], x[k + 6], x[k + 7]));
+            continue;
           }
           uint4 w[4];
 #pragma unroll
@@ -346,10 +420,11 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       bool ok = true;
       for (uint32_t k_item = 0; ok; ++k_item) {
         if (!mbar_wait(&sm.item_full[k_item % ITEMS], (k_item / ITEMS) & 1u, abort_flag)) { ok = false; break; }
-        const TilesItem it = sm.item[k_item % ITEMS];
+        const TilesItem& it = sm.item[k_item % ITEMS];
+        const bool go = it.go;
+        const int n0 = blocks_of(0, it), n1 = blocks_of(1, it), nmax = it.blocks;
         mbar_arrive(&sm.item_empty[k_item % ITEMS]);
-        if (!it.go) break;
-        const int n0 = blocks_of(it.row0, it.n, it.len), n1 = blocks_of(it.row0 + TM, it.n, it.len), nmax = max(n0, n1);
+        if (!go) break;
         if (!mbar_wait(&sm.q_full, k_item & 1u, abort_flag)) { ok = false; break; }
         if (nmax > 0) {
           if (!mbar_wait(&sm.k_full[blocks & 1u], (blocks >> 1) & 1u, abort_flag)) { ok = false; break; }
@@ -425,32 +500,50 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     __syncwarp();
   } else if (warp == 9) {
     // ------------------------------------------------------------------ items, pages, scales
-    // Items are dealt round-robin, the last rows of a head (under a causal mask the longest) first.  Lane g < 8 looks after
-    // a block's keys 16 g .. 16 g + 15; the next block's pages and scales are asked for before this one's are used.
+    // Lane g < 8 looks after a block's keys 16 g .. 16 g + 15; the next block's pages and scales are asked for before this
+    // one's are used.
     reg_dealloc<TILES_REGS_OTHER>();
-    int64_t left = blockIdx.x;              // items between the walk's place and this block's next item
-    int req = 0;
+    int req = 0, head = 0, pair = 0, block0 = 0;         // the walk's place: the next unit to be done
+    Request r{0, 0, 0};
+    if (units > 0) {
+      req = sm.start_i;
+      r = request_of(p, req);
+      const int64_t per_head = head_units(p, r);
+      head = static_cast<int>(sm.start_off / per_head);
+      int64_t off = sm.start_off - head * per_head;
+      for (;; ++pair) {
+        const int n = max(1, pair_blocks(p, pair * 2 * TM, r.n, r.len));
+        if (off < n) break;
+        off -= n;
+      }
+      block0 = static_cast<int>(off);
+    }
+    int done = 0;                           // units
     uint32_t blocks = 0;
     bool ok = true;
     for (uint32_t k_item = 0; ok; ++k_item) {
-      Request r{0, 0, 0};
-      bool go = false;
-      for (; req < p.B; ++req) {
-        r = request_of(p, req);
-        const int64_t n = request_items(p, r);
-        if (left < n) {
-          go = true;
-          break;
-        }
-        left -= n;
-      }
-      const int pairs = max(1, (r.n * p.G + 2 * TM - 1) / (2 * TM)), idx = static_cast<int>(left);
-      const int head = idx / pairs, row0 = (pairs - 1 - idx % pairs) * 2 * TM;
-      left += gridDim.x;
+      const bool go = done < units;
+      const int row0 = pair * 2 * TM;
+      const int in_item = go ? pair_blocks(p, row0, r.n, r.len) : 0, item_units = max(1, in_item);
+      const int take = go ? min(item_units - block0, units - done) : 0;
+      const int nmax = go ? min(take, in_item - block0) : 1;             // key blocks (none, where the pair sees nothing)
+      const bool whole = block0 == 0 && take == item_units;
       if (!mbar_wait(&sm.item_empty[k_item % ITEMS], ((k_item / ITEMS) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
       if (lane == 0) {
-        sm.item[k_item % ITEMS] = TilesItem{r.t0, r.n, r.len, head, row0, go, {0, 0}};
+        const int slot = k_item == 0 ? 0 : 1;
+        sm.item[k_item % ITEMS] = TilesItem{r.t0, r.n, r.len, head, row0, go, block0, max(nmax, 0), whole ? -1 : static_cast<int>(blockIdx.x) * 2 + slot, {0, 0, 0}};
         mbar_arrive(&sm.item_full[k_item % ITEMS]);
+        if (go && !whole && block0 == 0) {   // the item begins here and ends in a later block's range: this one lists the parts
+          const int64_t grid = min(static_cast<int64_t>(gridDim.x), total), last_unit = first_unit + done + item_units - 1;
+          int* meta = p.meta + blockIdx.x * 8;
+          meta[1] = static_cast<int>(((last_unit + 1) * grid - 1) / total);
+          meta[2] = slot;
+          meta[3] = r.t0;
+          meta[4] = r.n;
+          meta[5] = head;
+          meta[6] = row0;
+          meta[0] = 1;
+        }
       }
       // the item's queries on their way to L2
       for (int R = row0 + lane; go && R < min(row0 + 2 * TM, r.n * p.G); R += 32) {
@@ -459,11 +552,10 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
         for (int k = 0; k < D; k += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + k));
       }
-      const int nmax = go ? max(blocks_of(row0, r.n, r.len), blocks_of(row0 + TM, r.n, r.len)) : 1;
       int pid = -1, row = 0;
       float ks = 0.f, vs = 0.f;
       auto look_up = [&](int j) {
-        const int key = j * BN + 16 * lane;
+        const int key = (block0 + j) * BN + 16 * lane;
         pid = -1;
         ks = vs = 0.f;
         if (go && lane < 8 && j < nmax && key < r.len) {
@@ -504,7 +596,8 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const float fk = there ? rest(ks_now, ek, kref) : 1.f, fv = there ? rest(vs_now, ev, vnow) : 1.f;
         const uint32_t gone = __ballot_sync(0xffffffffu, page == -2);
         const bool plain = __all_sync(0xffffffffu, page != -2 && fk == 1.f);
-        const bool whole = gone == 0 && r.len - j * BN >= BN;
+        const int have = r.len - (block0 + j) * BN;
+        const bool full = gone == 0 && have >= BN;
         const bool unit_k = __all_sync(0xffffffffu, !there || ek == kref), unit_v = __all_sync(0xffffffffu, !there || ev == vnow);
         const bool plain_v = __all_sync(0xffffffffu, fv == 1.f);
         if (!mbar_wait(&sm.raw_empty[0], (b & 1u) ^ 1u, abort_flag)) { ok = false; break; }
@@ -521,9 +614,9 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           rec.vshift = j == 0 || vold == vexp ? 1.f : (vold == -1000 ? pow2f(-vexp) : pow2f(vold - vexp));
           rec.plain = plain;
           rec.gone = gone;
-          rec.mode[0] = !whole ? 2 : (unit_k ? 0 : 1);
-          rec.mode[1] = !whole || !plain_v ? 2 : (unit_v ? 0 : 1);
-          rec.have = go ? min(r.len - j * BN, BN) : -1;
+          rec.mode[0] = !full ? 2 : (unit_k ? 0 : 1);
+          rec.mode[1] = !full || !plain_v ? 2 : (unit_v ? 0 : 1);
+          rec.have = go ? min(have, BN) : -1;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.rec_full[b % RECORDS]);
@@ -541,7 +634,21 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (!ok) break;
       }
       if (!go) break;
-      blocks += nmax;
+      blocks += max(nmax, 0);
+      done += take;
+      block0 += take;
+      if (block0 == item_units) {           // on to the next pair, head, request
+        block0 = 0;
+        if (++pair == pairs_of(p, r)) {
+          pair = 0;
+          if (++head == p.Hkv) {
+            head = 0;
+            if (done < units)
+              do r = request_of(p, ++req);
+              while (r.n == 0);
+          }
+        }
+      }
     }
     if (!ok) {
       give_up();
@@ -558,8 +665,8 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     // the swizzle is the same in every row it meets and its addresses differ by constants.
     reg_dealloc<TILES_REGS_OTHER>();
     constexpr int CPR = D / 16;             // pieces of a row
-    constexpr int STEP = CONVERT_WARPS * 32 / CPR, PIECES = (BN + STEP - 1) / STEP;
-    static_assert(STEP % 8 == 0, "");
+    constexpr int STEP = CONVERT_WARPS * 32 / CPR, PIECES = BN / STEP;
+    static_assert(STEP % 8 == 0 && BN % STEP == 0 && PIECES % 4 == 0, "");
     const int ct = tid - (TILES_THREADS - CONVERT_WARPS * 32), r0 = ct / CPR, ch = ct % CPR;
     // The two 128-byte lines a row of D = 128 becomes share banks: threads of the second write their halves in the other order.
     const int swap = D == 128 ? ch >> 2 : 0;
@@ -582,41 +689,47 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const uint32_t src = src0 + side * (BN * D), dst = dst0 + (side * 2 + slot) * TILE;
         auto convert = [&](auto how) {
           constexpr int kMode = decltype(how)::value;
+#pragma unroll 1
+          for (int x0 = 0; x0 < PIECES; x0 += 4) {       // four pieces at once: the loads first
+            uint32_t w[4][2][2];
 #pragma unroll
-          for (int x = 0; x < PIECES; ++x) {
-            const int r = r0 + STEP * x;
-            if (STEP * x + STEP > BN && r >= BN) break;
-            uint32_t w[2][2], h[2][4];
-            lds64(src + x * STEP * D, w[0]);
-            lds64((src + x * STEP * D) ^ 8u, w[1]);
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int y = 0; y < 2; ++y) e4m3x4_to_f16(w[e][y], h[e][2 * y], h[e][2 * y + 1]);
-            if constexpr (kMode > 0) {
-              const uint32_t f = (side ? rec.rv : rec.rk)[r >> 4];
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int y = 0; y < 4; ++y) h[e][y] = hmul2(h[e][y], f);
+            for (int x = 0; x < 4; ++x) {
+              lds64(src + (x0 + x) * STEP * D, w[x][0]);
+              lds64((src + (x0 + x) * STEP * D) ^ 8u, w[x][1]);
             }
-            if constexpr (kMode == 2) {
-              const float fv = side ? rec.fv[r >> 4] : 1.f;
-              const bool nothing = r >= have || ((gone >> (r >> 4)) & 1u);   // (the bytes may be anything)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int r = r0 + STEP * (x0 + x);
+              uint32_t h[2][4];
 #pragma unroll
               for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                  uint32_t v = h[e][y];
-                  if (fv != 1.f) {
-                    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v));
-                    v = pack_f16(a.x * fv, a.y * fv);
+                for (int y = 0; y < 2; ++y) e4m3x4_to_f16(w[x][e][y], h[e][2 * y], h[e][2 * y + 1]);
+              if constexpr (kMode > 0) {
+                const uint32_t f = (side ? rec.rv : rec.rk)[r >> 4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                  for (int y = 0; y < 4; ++y) h[e][y] = hmul2(h[e][y], f);
+              }
+              if constexpr (kMode == 2) {
+                const float fv = side ? rec.fv[r >> 4] : 1.f;
+                const bool nothing = r >= have || ((gone >> (r >> 4)) & 1u);   // (the bytes may be anything)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                  for (int y = 0; y < 4; ++y) {
+                    uint32_t v = h[e][y];
+                    if (fv != 1.f) {
+                      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v));
+                      v = pack_f16(a.x * fv, a.y * fv);
+                    }
+                    h[e][y] = nothing ? 0u : v;
                   }
-                  h[e][y] = nothing ? 0u : v;
-                }
+              }
+              sts128(dst + (x0 + x) * STEP * 128 + first, h[0]);
+              sts128(dst + (x0 + x) * STEP * 128 + second, h[1]);
             }
-            sts128(dst + x * STEP * 128 + first, h[0]);
-            sts128(dst + x * STEP * 128 + second, h[1]);
           }
         };
         const int mode = rec.mode[side];
@@ -642,14 +755,80 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   }
 }
 
+// Merges the parts of items that several blocks worked on: a warp takes a row of an item at a time, in a fixed order.
 template <typename T, int D>
-int launch_tiles(const CachedParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV, cudaStream_t stream) {
+__global__ void __launch_bounds__(JWARPS * 32) cached_tiles_join_kernel(const CachedParams p, int blocks) {
+  __shared__ uint16_t s_block[MAX_TEAMS];             // blocks whose last item goes on behind them
+  __shared__ int s_count[JWARPS];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int items = open_items(p, blocks, s_block, s_count);
+  constexpr int VL = D / 32;                          // floats of a lane
+  const int warps = gridDim.x * JWARPS;
+  for (int job = blockIdx.x * JWARPS + warp; job < items * 2 * TM; job += warps) {
+    const int c0 = s_block[job / (2 * TM)], r = job % (2 * TM);
+    const int4* meta = reinterpret_cast<const int4*>(p.meta + c0 * 8);   // set, last block, slot, t0; n, head, row0
+    const int4 a = meta[0], b = meta[1];
+    const int R = b.z + r;
+    if (R >= b.x * p.G) continue;
+    float m = -INFINITY, l = 0.f, acc[VL];
+#pragma unroll
+    for (int k = 0; k < VL; ++k) acc[k] = 0.f;
+    for (int c = c0; c <= a.y; c += 4) {              // four parts asked for at once
+      float2 ml[4];
+      float v[4][VL];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t row = (static_cast<int64_t>(c + e) * 2 + (c + e == c0 ? a.z : 0)) * 2 * TM + r;
+        const bool in = c + e <= a.y;
+        ml[e] = in ? *reinterpret_cast<const float2*>(p.part_ml + row * 2) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int k = 0; k < VL; ++k) v[e][k] = in ? p.part_o[row * D + k * 32 + lane] : 0.f;
+      }
+      const float top = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x)), base = top == -INFINITY ? 0.f : top;
+      const float keep = exp2f_approx(m - base);
+      m = top;
+      l *= keep;
+#pragma unroll
+      for (int k = 0; k < VL; ++k) acc[k] *= keep;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float w = exp2f_approx(ml[e].x - base);
+        l = fmaf(ml[e].y, w, l);
+#pragma unroll
+        for (int k = 0; k < VL; ++k) acc[k] = fmaf(v[e][k], w, acc[k]);
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const int token = R / p.G;
+    T* dst = static_cast<T*>(p.O) + (a.w + token) * p.o_st + (b.y * p.G + R - token * p.G) * p.o_sh;
+#pragma unroll
+    for (int k = 0; k < VL; ++k) dst[k * 32 + lane] = Conv<T>::from_f(acc[k] * inv);
+  }
+}
+
+// Two parts per block, each 256 rows of D sums and (m, l), and eight ints per block.
+size_t tiles_workspace(int64_t D, int blocks) { return static_cast<size_t>(blocks) * (2 * 2 * TM * (D + 2) * 4 + 32); }
+
+template <typename T, int D>
+int launch_tiles(CachedParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV, void* workspace, cudaStream_t stream) {
   constexpr int SMEM = sizeof(TilesSmem<D>) + 1024;
   static_assert(SMEM <= 227 * 1024, "a block does not fit an SM's shared memory");
-  auto kern = cached_tiles_kernel<T, D>;
+  const int blocks = sm_count();
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + static_cast<size_t>(blocks) * 2 * 2 * TM * D;
+  p.meta = reinterpret_cast<int*>(p.part_ml + static_cast<size_t>(blocks) * 2 * 2 * TM * 2);
   static std::atomic<uint64_t> done{0};
-  const int rc = once_per_device(done, []() { return cudaFuncSetAttribute(cached_tiles_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM); });
+  int rc = once_per_device(done, []() {
+    const cudaError_t e = cudaFuncSetAttribute(cached_tiles_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(cached_tiles_join_kernel<T, D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+  });
   if (rc) return rc;
-  kern<<<sm_count(), TILES_THREADS, SMEM, stream>>>(tmK, tmV, p, make_idesc(0, 0, 0, 0, TM, BN), make_idesc(0, 0, 0, 1, TM, D));
-  return check_launch("cached_tiles_kernel");
+  if (blocks > MAX_TEAMS) return fail(KCG_ERR_UNSUPPORTED, "fmha_cached: a device of %d SMs", blocks);
+  cached_tiles_kernel<T, D><<<blocks, TILES_THREADS, SMEM, stream>>>(tmK, tmV, p, make_idesc(0, 0, 0, 0, TM, BN), make_idesc(0, 0, 0, 1, TM, D));
+  rc = check_launch("cached_tiles_kernel");
+  if (rc) return rc;
+  launch_overlapped(cached_tiles_join_kernel<T, D>, dim3(4 * blocks), dim3(JWARPS * 32), 0, stream, p, blocks);
+  return check_launch("cached_tiles_join_kernel");
 }
