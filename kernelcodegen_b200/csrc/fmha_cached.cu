@@ -58,6 +58,7 @@ struct CachedParams {
   int64_t T, uniform, num_pages;
   int B, Hkv, G, page, causal;
   int wk_log2;                      // 2^wk_log2 warps share a head's keys, the others take further heads
+  int whole_items;                  // the many-row kernel: items are dealt whole, not in ranges of key blocks
   int o_by_32;                      // rows of O start on 32-byte boundaries
   int box;                          // rows of a TMA box: 32 where a page is a multiple of that, else 16
   float scale_log2;
@@ -1061,7 +1062,10 @@ int launch_cached(CachedParams& p, int64_t rows, const CUtensorMap& tmK, const C
   // Two heads side by side where there are two: as fast as four or one with a head's page in one piece, and 20 % faster
   // than one where a token's heads stand together (8 x 4096 tokens of 32 heads, token-major: 54.8 us, one head 68.2).
   p.wk_log2 = p.Hkv % 2 == 0 ? 1 : 2;
-  if (rows > 16) return launch_tiles<T, D>(p, tmK, tmV, workspace, stream);
+  // Up to 48 rows the split kernel reads the cache once per 16 of them and is still faster than a 256-row item that is
+  // mostly empty: 16 requests x 4000 keys x 8 heads, 32 rows 73 against 112 us, 64 rows 125 against 113; 64 x 1000 keys 85
+  // against 134 and 148 against 137.
+  if (rows > 48) return launch_tiles<T, D>(p, items * ((rows + 255) / 256), tmK, tmV, workspace, stream);
   if (rows <= 8) return launch_split<T, D, 1>(p, tmK, tmV, items, workspace, stream);
   return launch_split<T, D, 2>(p, tmK, tmV, items * ((rows + 15) / 16), workspace, stream);
 }
