@@ -28,7 +28,7 @@ namespace {
 // block waits for another.
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxRequests = 16384;   // 12 bytes of shared memory each
-constexpr int kPlanTokensPerBlock = 2048; // 4 tokens per thread; measured in the notes at launch_plan
+constexpr int kPlanTokensPerBlock = 2048; // 4 tokens per thread
 
 struct PlanParams {
   const int32_t* cached;
@@ -153,17 +153,20 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const PlanPara
 
 // ---- appending ------------------------------------------------------------------------------------
 // Neighbouring tokens of one page in ascending slots, with fewer than 32 skipped tokens between two of
-// them, form a run; one warp writes a run of one head of K or V.  With amax the largest finite magnitude of the run,
+// them, form a run.  A run of one head of K or V is written by one warp, or by the four of a block where it has more rows
+// than a warp holds.  With amax the largest finite magnitude of the run,
 //   s = 2^k, the smallest power of two with amax / s <= 448 (e4m3's largest value), k >= -110;
 // a run that does not begin at its page's first row keeps max(s, old scale), and the rows before it are
 // rounded again when the scale has grown.  The scale is a power of two because e4m3 has an exponent of
 // its own: a finer scale would gain no significant bit, and x / s, code * s and a change of scale are
 // then exact, so that the only rounding is the one to e4m3's four significant bits.
 //
-// Bound by memory: each 16-bit element is read once and leaves as one byte.  A warp keeps its run in
-// registers between finding amax and rounding (up to kVecs 16-byte vectors per lane: 64 rows of
-// D = 128), with all of its loads in flight at once; longer runs are read twice.
-constexpr int kVecs = 32;
+// Bound by memory: each 16-bit element is read once and leaves as one byte.  A run stays in registers between
+// finding amax and rounding (up to kVecs 16-byte vectors per lane: 64 rows of D = 128 in a block), with all
+// of its loads in flight at once; longer runs are read twice.  8 prompts of 4096 tokens, 8 heads of 128: 51 us, 0.60 of the
+// copy rate (one warp per run with 32 vectors per lane left six warps on an SM: 83 us).  What is left is latency: slots,
+// old scale and rows are three trips to memory, and five blocks of four warps are in flight on an SM.
+constexpr int kVecs = 8;
 constexpr int kAppendWarps = 4;
 
 struct AppendSide {
@@ -177,7 +180,8 @@ struct AppendParams {
   AppendSide side[2];     // K, V
   const int64_t* slots;
   int64_t T, slot_end;    // slots are in [0, slot_end)
-  int heads, page, chunk; // tokens one warp looks at
+  int heads, page, chunk; // chunk: tokens one block looks at
+  int per;                // of the 2 * heads sides and heads, what one block writes
   int* status;
 };
 
@@ -231,154 +235,204 @@ __device__ __forceinline__ void encode(const uint4& v, float inv, uint32_t (&cod
     code[i] = to_e4m3x2(f[4 * i], f[4 * i + 1]) | (to_e4m3x2(f[4 * i + 2], f[4 * i + 3]) << 16);
 }
 
-// `slots`: of the run's first token, at row `off` of the page whose slots begin at `slot0`; it ends n tokens
-// later.  `dense`: nothing is skipped, token r goes to row off + r.
+// A page's first `off` rows, from scale `old` to `scale`: `parts` warps, this one is `part`.
+template <int D>
+__device__ __forceinline__ void round_again(uint8_t* rows, int64_t stride, int off, float old, float scale, int lane, int part, int parts) {
+  const float ratio = old / scale;
+  for (int r = part * (128 / D) + lane / (D / 4); r < off; r += parts * (128 / D)) {
+    uint32_t* q = reinterpret_cast<uint32_t*>(rows + r * stride) + lane % (D / 4);
+    const uint32_t w = *q;
+    uint32_t o = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * k)), __NV_E4M3);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+      o |= to_e4m3x2(f.x * ratio, f.y * ratio) << (16 * k);
+    }
+    *q = o;
+  }
+}
+template <int CW> __device__ __forceinline__ void store_codes(uint8_t* q, const uint32_t (&code)[CW]) {
+  if constexpr (CW == 2) *reinterpret_cast<uint2*>(q) = make_uint2(code[0], code[1]);
+  else *reinterpret_cast<uint32_t*>(q) = code[0];
+}
+
+// What a run is: a block finds it once for all heads.
+struct Run {
+  int64_t slot0, page;    // of the page
+  int at, n, off, dense;  // first token in the block's chunk, tokens, first row; dense: token r goes to row off + r
+};
+
+// The rare run, by one warp and a vector at a time: tokens are left out, or there are infinities or NaN.
 template <typename T, int D>
-__device__ __forceinline__ void append_run(const AppendSide& a, int head, int heads, const int64_t* slots, int64_t t0, int n,
-                                           bool dense, int64_t page, int64_t slot0, int page_size, int off, int lane) {
+__device__ __forceinline__ void append_odd(const AppendSide& a, int head, int heads, const int64_t* slots, int64_t t0, const Run& run, int page_size, int lane) {
+  constexpr int VE = 16 / sizeof(T), VR = D / VE, RPI = 32 / VR, CW = 4 / sizeof(T);
+  const int col = lane % VR;
+  const T* x = static_cast<const T*>(a.x) + t0 * a.st + head * a.sh + col * VE;
+  uint8_t* rows = a.cache + run.page * a.cp + head * a.ch;
+  float* sp = a.scale + run.page * heads + head;
+  const float old = run.off ? *sp : 0.f;
+  float amax = 0.f;
+  for (int r = lane / VR; r < run.n; r += RPI) {
+    const int64_t s = slots[r] - run.slot0;
+    if (s < 0 || s >= page_size) continue;
+    for (int e = 0; e < VE; ++e) {
+      const float f = fabsf(Conv<T>::to_f(x[r * a.st + e]));
+      if (f < INFINITY) amax = fmaxf(amax, f);
+    }
+  }
+  const float scale = fmaxf(exp2i(scale_exponent(warp_max(amax))), old), inv = 1.0f / scale;
+  if (run.off && scale != old) round_again<D>(rows, a.ct, run.off, old, scale, lane, 0, 1);
+  for (int r = lane / VR; r < run.n; r += RPI) {
+    const int64_t s = slots[r] - run.slot0;
+    if (s < 0 || s >= page_size) continue;
+    uint32_t code[CW];
+    encode<T, true>(*reinterpret_cast<const uint4*>(x + r * a.st), inv, code);
+    store_codes<CW>(rows + s * a.ct + col * VE, code);
+  }
+  if (lane == 0) *sp = scale;
+}
+
+// A dense run; kParts warps (this one is `part`) share it.  False: it has values that are not finite, and nothing was written.
+template <typename T, int D, int kParts>
+__device__ __forceinline__ bool append_run(const AppendSide& a, int head, int heads, int64_t t0, const Run& run, int lane, int part,
+                                           uint32_t* s_max) {
   constexpr int VE = 16 / sizeof(T);        // elements of a vector
   constexpr int VR = D / VE;                // vectors of a row
   constexpr int RPI = 32 / VR;              // rows one warp instruction covers
-  constexpr int CAP = kVecs * RPI;          // rows held in registers
+  constexpr int CAP = kVecs * RPI * kParts; // rows held in registers
   constexpr int CW = 4 / sizeof(T);         // words of codes per vector
-  const int sub = lane / VR, col = lane % VR;
-  const T* x = static_cast<const T*>(a.x) + t0 * a.st + head * a.sh + col * VE;
-  uint8_t* out = a.cache + page * a.cp + head * a.ch + col * VE;
-  float* sp = a.scale + page * heads + head;
-  const float old = off ? *sp : 0.f;        // a run at a page's first row: the page is new
-
-  auto row_of = [&](int r) -> int {         // where token r of the run goes, -1: nowhere
-    if (r >= n) return -1;
-    if (dense) return off + r;
-    const int64_t s = slots[r] - slot0;
-    return s >= 0 && s < page_size ? static_cast<int>(s) : -1;
-  };
+  const int first = part * RPI + lane / VR, col = lane % VR, n = run.n;
+  const T* x = static_cast<const T*>(a.x) + (t0 + first) * a.st + head * a.sh + col * VE;
+  const int64_t x_step = a.st * (RPI * kParts), out_step = a.ct * (RPI * kParts);
+  uint8_t* rows = a.cache + run.page * a.cp + head * a.ch;
+  float* sp = a.scale + run.page * heads + head;
+  const float old = run.off ? *sp : 0.f;    // a run at a page's first row: the page is new
   uint4 v[kVecs];
   auto load = [&](int base) {
+    const T* at = x + base * a.st;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      if (i % 4 == 0 && base + i * RPI >= n) break;
-      const int r = base + i * RPI + sub;
-      v[i] = row_of(r) >= 0 ? __ldcs(reinterpret_cast<const uint4*>(x + r * a.st)) : make_uint4(0, 0, 0, 0);
-    }
+    for (int i = 0; i < kVecs; ++i, at += x_step)
+      v[i] = base + first + i * RPI * kParts < n ? __ldcs(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
   };
   uint32_t mag = 0;
   for (int base = 0; base < n; base += CAP) {
     load(base);
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      if (i % 4 == 0 && base + i * RPI >= n) break;
-      mag = mag_max<T>(mag_max<T>(mag_max<T>(mag_max<T>(mag, v[i].x), v[i].y), v[i].z), v[i].w);
-    }
+    for (int i = 0; i < kVecs; ++i) mag = mag_max<T>(mag_max<T>(mag_max<T>(mag_max<T>(mag, v[i].x), v[i].y), v[i].z), v[i].w);
   }
   if (sizeof(T) == 2) mag = max(mag & 0xffffu, mag >> 16);
   mag = __reduce_max_sync(0xffffffffu, mag);
-  const bool special = mag >= MagInf<T>::v;
-  float amax = mag_to_float<T>(mag);
-  if (special) {                            // rare: leave infinities and NaN out of amax
-    amax = 0.f;
-    for (int r = sub; r < n; r += RPI)
-      for (int e = 0; e < VE && row_of(r) >= 0; ++e) {
-        const float f = fabsf(Conv<T>::to_f(x[r * a.st + e]));
-        if (f < INFINITY) amax = fmaxf(amax, f);
-      }
-    amax = warp_max(amax);
-  }
-  const float want = exp2i(scale_exponent(amax));
-  const float scale = fmaxf(want, old);
-  if (off && scale != old) {                // the page's earlier rows: from the old scale to the new one
-    const float ratio = old / scale;
-    for (int r = lane / (D / 4); r < off; r += 32 / (D / 4)) {
-      uint32_t* q = reinterpret_cast<uint32_t*>(a.cache + page * a.cp + head * a.ch + static_cast<int64_t>(r) * a.ct) +
-                    lane % (D / 4);
-      const uint32_t w = *q;
-      uint32_t o = 0;
+  if (kParts > 1) {
+    __syncthreads();                        // the values of the run before have been read
+    if (lane == 0) s_max[part] = mag;
+    __syncthreads();
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * k)), __NV_E4M3);
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-        o |= to_e4m3x2(f.x * ratio, f.y * ratio) << (16 * k);
-      }
-      *q = o;
-    }
+    for (int w = 0; w < kParts; ++w) mag = max(mag, s_max[w]);
   }
-  // a power of two, unless the caller's own scale is kept
-  const float inv = 1.0f / scale;
+  if (mag >= MagInf<T>::v) return false;    // (the same answer in all of the run's warps)
+  const float scale = fmaxf(exp2i(scale_exponent(mag_to_float<T>(mag))), old);
+  if (run.off && scale != old) round_again<D>(rows, a.ct, run.off, old, scale, lane, part, kParts);
+  const float inv = 1.0f / scale;           // a power of two, unless the caller's own scale is kept
+  uint8_t* out = rows + (run.off + first) * a.ct + col * VE;
   for (int base = 0; base < n; base += CAP) {
     if (n > CAP) load(base);
+    uint8_t* at = out + base * a.ct;
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      if (i % 4 == 0 && base + i * RPI >= n) break;
-      const int r = base + i * RPI + sub;
+    for (int i = 0; i < kVecs; ++i, at += out_step) {
       uint32_t code[CW];
-      if (special) encode<T, true>(v[i], inv, code); else encode<T, false>(v[i], inv, code);
-      const int row = row_of(r);
-      if (row >= 0) {
-        uint8_t* q = out + static_cast<int64_t>(row) * a.ct;
-        if constexpr (CW == 2) *reinterpret_cast<uint2*>(q) = make_uint2(code[0], code[1]);
-        else *reinterpret_cast<uint32_t*>(q) = code[0];
-      }
+      encode<T, false>(v[i], inv, code);
+      if (base + first + i * RPI * kParts < n) store_codes<CW>(at, code);
     }
   }
-  if (lane == 0 && (!off || scale != old)) *sp = scale;
+  if (lane == 0 && part == 0 && (!run.off || scale != old)) *sp = scale;
+  return true;
 }
 
+// Finding the runs costs more than a head's share of a short run, so one warp finds a block's and the block writes them for
+// several heads.
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kAppendWarps) cache_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(32 * kAppendWarps, 5) cache_append_kernel(const AppendParams p) {
   grid_launch_dependents();
   grid_dependency_wait();
-  const int lane = threadIdx.x & 31;
-  const int64_t chunk = static_cast<int64_t>(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
-  const int head = blockIdx.y % p.heads;
-  const AppendSide& a = p.side[blockIdx.y / p.heads];
-  const int64_t t0 = chunk * p.chunk;
-  if (t0 >= p.T) return;
+  __shared__ Run s_run[32];
+  __shared__ int s_runs;
+  __shared__ uint32_t s_max[kAppendWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * p.chunk;
   const int count = static_cast<int>(min(static_cast<int64_t>(p.chunk), p.T - t0));   // <= 32
-
-  auto in_pool = [&](int64_t s) { return s >= 0 && s < p.slot_end; };
-  int64_t slot = -1, before = -1;
-  if (lane < count) {
-    slot = p.slots[t0 + lane];
-    if (!in_pool(slot) && slot != -1 && p.status) *p.status = KCG_ERR_INVALID_ARG;
-  }
-  const bool valid = in_pool(slot);
-  if (valid)                                // the last token before this one that is not skipped
-    for (int64_t k = t0 + lane - 1; k >= 0 && k > t0 + lane - 33 && !in_pool(before); --k) before = p.slots[k];
-  const int64_t page = valid ? slot / p.page : -1;
-  const bool first = valid && !(in_pool(before) && before < slot && before / p.page == page);   // of a run
-  for (uint32_t left = __ballot_sync(0xffffffffu, first); left; left &= left - 1) {
-    const int at = __ffs(left) - 1;
-    const int64_t s0 = __shfl_sync(0xffffffffu, slot, at), page0 = __shfl_sync(0xffffffffu, page, at);
-    const int64_t slot0 = page0 * p.page, tr = t0 + at;
-    // the run's last token, looking 32 tokens on from the last one found
-    int n = 1, found = 1;
-    int64_t s_last = s0;
-    for (bool more = true; more;) {
-      const int64_t k = tr + n + lane;
-      const int64_t s = k < p.T ? p.slots[k] : -1;
-      const bool in = in_pool(s);
-      const uint32_t others = __ballot_sync(0xffffffffu, in && !(s > s0 && s < slot0 + p.page));
-      uint32_t ours = __ballot_sync(0xffffffffu, in && s > s0 && s < slot0 + p.page);
-      if (others) ours &= (1u << (__ffs(others) - 1)) - 1;
-      more = ours != 0 && others == 0 && n < p.T;
-      if (ours) {
-        const int top = 31 - __clz(ours);
-        s_last = __shfl_sync(0xffffffffu, s, top);
-        found += __popc(ours);
-        n += top + 1;
-      }
+  if (warp == 0) {
+    auto in_pool = [&](int64_t s) { return s >= 0 && s < p.slot_end; };
+    auto page_of = [&](int64_t s) -> int64_t {   // (a 64-bit division is several times a 32-bit one)
+      return p.slot_end <= UINT32_MAX ? static_cast<int64_t>(static_cast<uint32_t>(s) / static_cast<uint32_t>(p.page)) : s / p.page;
+    };
+    int64_t slot = -1, before = -1;
+    if (lane < count) {
+      slot = p.slots[t0 + lane];
+      if (!in_pool(slot) && slot != -1 && p.status) *p.status = KCG_ERR_INVALID_ARG;
     }
-    // ascending slots of one page: nothing is left out when they span as many as they are
-    const bool dense = found == n && s_last == s0 + n - 1;
-    append_run<T, D>(a, head, p.heads, p.slots + tr, tr, n, dense, page0, slot0, p.page, static_cast<int>(s0 - slot0), lane);
+    const bool valid = in_pool(slot);
+    if (valid)                              // the last token before this one that is not skipped
+      for (int64_t k = t0 + lane - 1; k >= 0 && k > t0 + lane - 33 && !in_pool(before); --k) before = p.slots[k];
+    const int64_t page = valid ? page_of(slot) : -1;
+    const bool first = valid && !(in_pool(before) && before < slot && page_of(before) == page);   // of a run
+    int runs = 0;
+    for (uint32_t left = __ballot_sync(0xffffffffu, first); left; left &= left - 1, ++runs) {
+      const int at = __ffs(left) - 1;
+      const int64_t s0 = __shfl_sync(0xffffffffu, slot, at), page0 = __shfl_sync(0xffffffffu, page, at);
+      const int64_t slot0 = page0 * p.page, tr = t0 + at;
+      // the run's last token, looking 32 tokens on from the last one found
+      int n = 1, found = 1;
+      int64_t s_last = s0;
+      for (bool more = true; more;) {
+        const int64_t k = tr + n + lane;
+        const int64_t s = k < p.T ? p.slots[k] : -1;
+        const bool in = in_pool(s);
+        const uint32_t others = __ballot_sync(0xffffffffu, in && !(s > s0 && s < slot0 + p.page));
+        uint32_t ours = __ballot_sync(0xffffffffu, in && s > s0 && s < slot0 + p.page);
+        if (others) ours &= (1u << (__ffs(others) - 1)) - 1;
+        more = ours != 0 && others == 0 && n < p.T;
+        if (ours) {
+          const int top = 31 - __clz(ours);
+          s_last = __shfl_sync(0xffffffffu, s, top);
+          found += __popc(ours);
+          n += top + 1;
+        }
+      }
+      // ascending slots of one page: nothing is left out when they span as many as they are
+      if (lane == 0) s_run[runs] = Run{slot0, page0, at, n, static_cast<int>(s0 - slot0), found == n && s_last == s0 + n - 1};
+    }
+    if (lane == 0) s_runs = runs;
+  }
+  __syncthreads();
+  const int runs = s_runs, h0 = blockIdx.y * p.per, mine = min(p.per, 2 * p.heads - h0);
+  constexpr int ALONE = kVecs * 32 / (D * static_cast<int>(sizeof(T)) / 16);   // rows one warp holds
+  int turn = 0;
+  for (int k = 0; k < runs; ++k) {
+    const Run& r = s_run[k];
+    for (int h = h0; h < h0 + mine; ++h) {
+      const AppendSide& a = p.side[h >= p.heads];
+      const int head = h >= p.heads ? h - p.heads : h;
+      const int64_t* slots = p.slots + t0 + r.at;
+      // a long run is the whole block's, short ones are dealt to the warps in turn
+      bool written = false, mine_too = warp == 0;
+      if (r.dense && r.n > ALONE) {
+        written = append_run<T, D, kAppendWarps>(a, head, p.heads, t0 + r.at, r, lane, warp, s_max);
+      } else {
+        mine_too = turn++ % kAppendWarps == warp;
+        if (mine_too && r.dense) written = append_run<T, D, 1>(a, head, p.heads, t0 + r.at, r, lane, 0, s_max);
+      }
+      if (!written && mine_too) append_odd<T, D>(a, head, p.heads, slots, t0 + r.at, r, p.page, lane);
+    }
   }
 }
 
 template <typename T>
 int launch_append(const AppendParams& p, int64_t D, cudaStream_t stream) {
-  const int64_t blocks = ((p.T + p.chunk - 1) / p.chunk + kAppendWarps - 1) / kAppendWarps;
-  if (blocks > INT32_MAX || 2 * p.heads > 65535) return fail(KCG_ERR_UNSUPPORTED, "cache_append: too many tokens or heads");
-  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(2 * p.heads)), block(32 * kAppendWarps);
+  const int64_t blocks = (p.T + p.chunk - 1) / p.chunk;
+  const int64_t shares = (2 * p.heads + p.per - 1) / p.per;
+  if (blocks > INT32_MAX || shares > 65535) return fail(KCG_ERR_UNSUPPORTED, "cache_append: too many tokens or heads");
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(shares)), block(32 * kAppendWarps);
   if (D == 128) launch_overlapped(cache_append_kernel<T, 128>, grid, block, 0, stream, p);
   else launch_overlapped(cache_append_kernel<T, 64>, grid, block, 0, stream, p);
   return check_launch("cache_append_kernel");
@@ -462,11 +516,12 @@ extern "C" int kcg_cache_append(int dtype, int64_t T, int64_t Hkv, int64_t D, co
   p.slot_end = num_pages * page_size;
   p.heads = static_cast<int>(Hkv);
   p.page = static_cast<int>(page_size);
-  // Tokens per warp: one while the warps of all tokens fit the GPU about twice over (a decode step is a
-  // chain of dependent loads, so every run wants a warp of its own), then up to 32.
-  const int64_t warps = static_cast<int64_t>(sm_count()) * 64;
-  int64_t chunk = (T * 2 * Hkv + warps - 1) / warps;
-  p.chunk = static_cast<int>(chunk < 1 ? 1 : (chunk > 32 ? 32 : chunk));
+  // Blocks enough to fill the GPU a few times over: first tokens are put together (a block looks at up to 32), then heads.
+  const int64_t blocks = static_cast<int64_t>(sm_count()) * 32;
+  const int64_t chunk = (T * 2 * Hkv + blocks - 1) / blocks;
+  p.chunk = static_cast<int>(chunk > 32 ? 32 : chunk);
+  const int64_t per = (T + p.chunk - 1) / p.chunk * 2 * Hkv / blocks;
+  p.per = static_cast<int>(per < 1 ? 1 : (per > 2 * Hkv ? 2 * Hkv : per));
   p.status = device_status_word();
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
