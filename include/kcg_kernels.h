@@ -543,13 +543,17 @@ KCG_API int kcg_cache_append(int dtype, int64_t T, int64_t Hkv, int64_t D, const
  * is read behind a request's last token.  Block table entries outside the pool are not followed:
  * their keys are left out, and kcg_device_status() reports KCG_ERR_INVALID_ARG, as it does for
  * lengths beyond the table (cut) and a cu_new that descends or leaves [0, T] (clamped).
- * max_new: the most rows a request has, as far as the caller knows (0: T); it chooses the kernel, and
- * a wrong value costs time only.
+ * max_new: the most rows a request has, as far as the caller knows (0: T / B is assumed); it chooses the
+ * kernel, and a wrong value costs time only.
  *
  * dtype of Q and O: KCG_BF16 or KCG_F16; D in {64, 128}; page_size a multiple of 16; any fp32
- * scales.  Statistics and sums are fp32, P is rounded to fp16.
- * `workspace`: kcg_fmha_cached_workspace bytes of the current device, 16-byte aligned, for this call
- * alone until it has run; its contents need not be kept or cleared.
+ * scales.  Statistics and sums are fp32, P is rounded to fp16.  With more than 48 rows per key head
+ * (max_new * Hq / Hkv) the codes are widened to fp16 relative to the largest scale among 128 keys (K)
+ * or among the keys up to there (V): a page whose scale lies more than 2^15 below loses low bits of
+ * its codes, one 2^34 below counts as zeros; and V times what its scale is beside a power of two is
+ * rounded to fp16.  Scales of kcg_cache_append are powers of two.
+ * `workspace`: kcg_fmha_cached_workspace bytes of the current device (39 MB with 148 SMs and D = 128),
+ * 16-byte aligned, for this call alone until it has run; its contents need not be kept or cleared.
  */
 KCG_API int kcg_fmha_cached_workspace(int64_t D, size_t* bytes);
 KCG_API int kcg_fmha_cached_fwd(int dtype, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,

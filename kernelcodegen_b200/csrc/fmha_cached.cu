@@ -26,6 +26,7 @@
 #include "common.cuh"
 #include "tcgen05.cuh"
 
+#include <algorithm>
 #include <atomic>
 #include <cstddef>
 #include <type_traits>
@@ -1142,7 +1143,7 @@ extern "C" int kcg_fmha_cached_fwd(int dtype, int64_t T, int64_t B, int64_t Hq, 
   int mrc = cache_map(&tmK, k_cache, kc_strides, D, p);
   if (!mrc) mrc = cache_map(&tmV, v_cache, vc_strides, D, p);
   if (mrc) return mrc;
-  const int64_t rows = (max_new > 0 ? max_new : (T + B - 1) / B) * p.G;
+  const int64_t rows = (max_new > 0 ? std::min(max_new, T) : (T + B - 1) / B) * p.G;
   if (dtype == KCG_BF16)
     return D == 128 ? launch_cached<__nv_bfloat16, 128>(p, rows, tmK, tmV, workspace, s) : launch_cached<__nv_bfloat16, 64>(p, rows, tmK, tmV, workspace, s);
   return D == 128 ? launch_cached<__half, 128>(p, rows, tmK, tmV, workspace, s) : launch_cached<__half, 64>(p, rows, tmK, tmV, workspace, s);

@@ -19,8 +19,9 @@
 //
 // tcgen05 multiplies f16 with f16 or e4m3 with e4m3, not one with the other, and P in e4m3 would keep four bits; so the
 // codes are widened on the way.  Scales: a page's is 2^e f with f in [1, 2).  The power of two, relative to the block's
-// largest (K) or the item's largest so far (V), is multiplied into the codes, exactly down to f16's smallest step (a
-// page would have to lie 2^20 below to lose a bit that counts); the references go into the softmax constant and the
+// largest (K) or the item's largest so far (V), is multiplied into the codes, exactly where a page lies up to
+// 2^15 below (e4m3's smallest step is 2^-9, f16's 2^-24); further down a code is off by up to 2^-25 of the reference, which
+// beside the reference's own codes is less than the f16 rounding of P.  The references go into the softmax constant and the
 // output.  Where some f is not 1 (scales this library did not write) the softmax multiplies the scores of a page's 16-key
 // groups with it, and V is multiplied with it, rounding once more, to f16.
 // Tensor memory (512 columns): S0, S1, O0, O1; P_i overwrites the first half of S_i.
@@ -63,7 +64,7 @@ template <int D> struct TilesSmem {
   BlockRecord rec[RECORDS];
   TilesItem item[ITEMS];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], rec_full[RECORDS], raw_full[2], raw_empty[2], item_full[ITEMS], item_empty[ITEMS];
-  uint64_t q_full, s_full[2], p_full[4], o_full[2], drain;
+  uint64_t q_full[2], s_full[2], p_full[4], o_full[2], drain;
   int64_t scan[16], start_off;
   int start_i;
   uint32_t tmem;
@@ -169,6 +170,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       mbar_init(&sm.k_empty[s], 1);
       mbar_init(&sm.v_full[s], CONVERT_WARPS);
       mbar_init(&sm.v_empty[s], 1);
+      mbar_init(&sm.q_full[s], 4);
       mbar_init(&sm.s_full[s], 1);
       mbar_init(&sm.o_full[s], 1);
       mbar_init(&sm.p_full[2 * s], 4);
@@ -179,7 +181,6 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       mbar_init(&sm.item_full[s], 1);
       mbar_init(&sm.item_empty[s], 9);      // eight softmax warps and the issuing thread
     }
-    mbar_init(&sm.q_full, 8);
     mbar_init(&sm.drain, 1);
     sm.abort = 0;
     mbar_fence_init();
@@ -309,7 +310,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.q_full);
+      if (lane == 0) mbar_arrive(&sm.q_full[i]);
       return factor * fabsf(p.scale_log2);
     };
     bool ok = true, have_q = false;
@@ -325,7 +326,9 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const int R = it.row0 + i * TM + r;
         if (R < it.n * p.G) seen = (p.causal ? min(it.len, it.len - it.n + 1 + R / p.G) : it.len) - it.block0 * BN;
       }
-      if (!have_q) {
+      // A tile without key blocks has no queries either: its warps run on to later items, up to the ring's length, and
+      // phases of q_full count the items that use them, which nobody can run ahead of.
+      if (!have_q && n_mine > 0) {
         fetch_q(it);
         c = convert_q();
       }
@@ -343,7 +346,8 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         if (j + 1 == n_mine) {
           // the tile's last scores are there, so its Q is free: the next item's, if that is known already
           const uint32_t next = k_item + 1;
-          if (__all_sync(0xffffffffu, mbar_try_wait(&sm.item_full[next % ITEMS], (next / ITEMS) & 1u)) && sm.item[next % ITEMS].go) {
+          if (__all_sync(0xffffffffu, mbar_try_wait(&sm.item_full[next % ITEMS], (next / ITEMS) & 1u)) && sm.item[next % ITEMS].go &&
+              blocks_of(i, sm.item[next % ITEMS]) > 0) {
             fetch_q(sm.item[next % ITEMS]);
             have_q = true;
           }
@@ -443,6 +447,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const uint32_t kf = smem_u32(sm.k_full), vf = smem_u32(sm.v_full), pf = smem_u32(sm.p_full), sf = smem_u32(sm.s_full),
                      of = smem_u32(sm.o_full);
       uint32_t blocks = 0, cp0 = 0, cp1 = 0;             // key blocks before this item, P blocks of the tiles so far
+      uint32_t q_phase = 0;                              // phases of q_full: bit i
       bool ok = true;
       for (uint32_t k_item = 0; ok; ++k_item) {
         if (!mbar_wait(&sm.item_full[k_item % ITEMS], (k_item / ITEMS) & 1u, abort_flag)) { ok = false; break; }
@@ -451,7 +456,13 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const int n0 = blocks_of(0, it), n1 = blocks_of(1, it), nmax = it.blocks;
         mbar_arrive(&sm.item_empty[k_item % ITEMS]);
         if (!go) break;
-        if (!mbar_wait(&sm.q_full, k_item & 1u, abort_flag)) { ok = false; break; }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if ((i == 0 ? n0 : n1) > 0) {
+            if (!mbar_wait(&sm.q_full[i], (q_phase >> i) & 1u, abort_flag)) ok = false;
+            q_phase ^= 1u << i;
+          }
+        if (!ok) break;
         if (nmax > 0) {
           if (!mbar_wait(&sm.k_full[blocks & 1u], (blocks >> 1) & 1u, abort_flag)) { ok = false; break; }
           tc_fence_after();

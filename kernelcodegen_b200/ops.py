@@ -506,7 +506,8 @@ def fmha_cached(Q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, cu_
     says where each begins, or None when all have T / B.  ``lengths`` (int32 [B]) counts a request's tokens in
     the cache, the new ones last; causal masks keys behind a row's own.  Returns O like Q; rows that see no
     key are zero, rows outside cu_new's range are left as they were in ``out`` (unspecified without ``out``).
-    ``max_new``: the most rows one request has, if the caller knows it; it only chooses the kernel."""
+    ``max_new``: the most rows one request has, if the caller knows it; it only chooses the kernel (and, above 48
+    rows per key head, the one whose f16 operands are relative to the largest page scale: see the C header)."""
     what = "fmha_cached"
     _check_cache(what, k_cache, v_cache, k_scale, v_scale)
     pages, Hkv, page_size, D = k_cache.shape
