@@ -174,3 +174,38 @@ def test_no_work_at_all():
         ops().fmha_cached(*args, i32([0, 0, 0, 0]).cuda(), softmax_scale=0.1, max_new=max_new, out=out)
         sync_ok()
         assert bool((out == 3).all())
+
+
+def test_cache_beyond_32_bit_offsets():
+    """The last pages of a pool of more than 2^32 bytes, through append and each attention kernel."""
+    pages, Hkv, page, D, n = 140000, 2, 128, 128, 300
+    assert pages * Hkv * page * D > 2 ** 32
+    k, v = (torch.zeros((pages, Hkv, page, D), dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+    ks, vs = (torch.ones((pages, Hkv), device="cuda") for _ in range(2))
+    ids = [pages - 1, 0, pages - 2]
+    slots = [ids[t // page] * page + t % page for t in range(n)]
+    g = torch.Generator().manual_seed(50)
+    Q, K, V = (torch.randn((n, h, D), generator=g).to(torch.bfloat16) for h in (4, Hkv, Hkv))
+    ops().cache_append(K.cuda(), V.cuda(), torch.tensor(slots).cuda(), k, v, ks, vs)
+    # the pages in use, renumbered
+    code = [x.view(torch.uint8)[ids].cpu().view(torch.float8_e4m3fn) for x in (k, v)]
+    scale = [x[ids].cpu() for x in (ks, vs)]
+    for x, c, s in ((K, code[0], scale[0]), (V, code[1], scale[1])):
+        want = torch.zeros((3, Hkv, page, D), dtype=torch.float64), torch.ones((3, Hkv), dtype=torch.float64)
+        R.append(x, list(range(n)), *want, page)
+        assert torch.equal(c.double(), want[0]) and torch.equal(s.double(), want[1])
+    for rows, max_new in ((n, MANY), (8, 8), (2, 2)):
+        c = dict(Q=Q[:rows], code=code, scale=scale, table=[[0, 1, 2]], lengths=[n], cu=[0, rows], page=page)
+        got = ops().fmha_cached(Q[:rows].cuda(), k, v, ks, vs, i32([ids]).cuda(), i32([n]).cuda(), softmax_scale=0.09, causal=True,
+                                max_new=max_new)
+        sync_ok()
+        check(c, got, 0.09, True, many=rows > 24)
+
+
+def test_table_without_columns():
+    c = make([0, 0], [1, 30], 16, 4, 2, 64, torch.float16, seed=51)
+    args = [*c["args"][:5], torch.empty((2, 0), dtype=torch.int32, device="cuda"), c["args"][6]]
+    for max_new in (1, 10, MANY):
+        got = ops().fmha_cached(*args, c["cu_dev"], softmax_scale=0.1, max_new=max_new)
+        sync_ok()
+        assert bool((got == 0).all())
