@@ -149,10 +149,11 @@ template <int ROWS> struct Cursor {
   }
 };
 
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+// 4 or 16 bytes, or as many zero bytes without a look at the source
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool take) {
+  const int bytes = take ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
-// 16 bytes, or sixteen zero bytes without a look at the source
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
   const int bytes = take ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -463,7 +464,8 @@ __device__ __forceinline__ void feed_team(const CachedParams& p, const CUtensorM
       if (lane < 16) {
         const int page = k & 1 ? page1_of : page0_of;
         float* dst = (k & 2 ? sm.entry[w][stage].vs : sm.entry[w][stage].ks) + (k & 1);
-        if (page >= 0) cp_async4(smem_u32(dst), (k & 2 ? p.vs : p.ks) + static_cast<int64_t>(page) * p.Hkv + head_of);
+        // (the scale of a half without keys is 0: it multiplies a product that is zero, and what stood there may be NaN)
+        cp_async4(smem_u32(dst), (k & 2 ? p.vs : p.ks) + (page >= 0 ? static_cast<int64_t>(page) * p.Hkv + head_of : 0), page >= 0);
         cp_async_arrive(&sm.full[w][stage]);
       }
     }
@@ -933,7 +935,7 @@ __global__ void __launch_bounds__(JWARPS * 32) cached_join_kernel(const CachedPa
     const bool mine = job < jobs;
     const int c0 = mine ? s_team[job / tiles] : 0;
     const int4 a = meta[2 * c0], b = meta[2 * c0 + 1];
-    const int parts = a.y - c0 + 1, n = b.x, rb = b.z, rows = n * p.G - rb * ROWS;
+    const int parts = mine ? a.y - c0 + 1 : 0, n = b.x, rb = b.z, rows = n * p.G - rb * ROWS;
     const int head_in_group = job % tiles / (NQ * MT), k = job % (NQ * MT), q = k / MT;
     const bool live0 = mine && 8 * q + 2 * t < rows, live1 = mine && 8 * q + 2 * t + 1 < rows;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, acc[1][4] = {{0.f, 0.f, 0.f, 0.f}};

@@ -1,6 +1,7 @@
 """The paged 8-bit key / value cache on the GPU: planning, appending and attention against their restatement in
 64 bits (tests/cache_reference.py).  Planning and appending are compared bit for bit; attention element by element
 within the error its arithmetic admits."""
+import ctypes
 import math
 import random
 
@@ -495,3 +496,39 @@ def test_two_streams_at_once():
     sync_ok()
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+@pytest.mark.parametrize("new", [1, 6])
+def test_attention_scales_of_other_requests_do_not_leak(new):
+    """A request whose scales are NaN shares a block's buffers with one whose last half tile holds no keys."""
+    B = 1200
+    c = make([32, 10] * (B // 2), [new] * B, 16, 4, 1, 64, torch.float16, seed=61)
+    want = ops().fmha_cached(*c["args"], c["cu_dev"], softmax_scale=0.1, causal=True, max_new=new)
+    ks, vs = c["args"][3].clone(), c["args"][4].clone()
+    for i in range(0, B, 2):
+        ks[c["table"][i][1]] = math.nan
+        vs[c["table"][i][1]] = math.nan
+    got = ops().fmha_cached(*c["args"][:3], ks, vs, *c["args"][5:], c["cu_dev"], softmax_scale=0.1, causal=True, max_new=new)
+    sync_ok()
+    got, want = got.view(B, new, 4, 64), want.view(B, new, 4, 64)
+    assert bool(torch.isnan(got[::2, -1]).all()) and torch.equal(got[1::2], want[1::2])
+
+
+@pytest.mark.parametrize("word", [-1, 0, 1, 2 ** 30, 2 ** 31 - 1, 0x7FC00000])
+def test_attention_workspace_may_hold_anything(word):
+    from kernelcodegen_b200 import _lib
+    size = ctypes.c_size_t()
+    assert _lib.load().kcg_fmha_cached_workspace(64, ctypes.byref(size)) == 0
+    for lengths, new in (([5, 200, 0, 3000], 1), ([40, 1000], 6), ([700, 60], 70)):
+        c = make(lengths, [new] * len(lengths), 16, 4, 2, 64, torch.float16, seed=62)
+        st2, st3 = (ctypes.c_int64 * 2)(256, 64), (ctypes.c_int64 * 3)(2048, 1024, 64)
+        work = torch.full((size.value // 4,), word, dtype=torch.int32, device="cuda")
+        Q, k, v, ks, vs, table, lens = c["args"]
+        out = torch.empty_like(Q)
+        rc = _lib.load().kcg_fmha_cached_fwd(_lib.F16, Q.shape[0], len(lengths), 4, 2, 64, new, 0.1, 1, Q.data_ptr(), st2, k.data_ptr(), st3,
+                                             ks.data_ptr(), v.data_ptr(), st3, vs.data_ptr(), k.shape[0], 16, table.data_ptr(),
+                                             table.shape[1], table.stride(0), lens.data_ptr(), None, out.data_ptr(), st2,
+                                             work.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        sync_ok()
+        check(c, out, 0.1, True, many=new * 2 > 48)
