@@ -26,6 +26,7 @@ namespace {
 // bytes.  Every thread block computes the whole prefix sum into its shared memory (a few loads per
 // thread) and then fills its own share of the tokens and requests, so a step is one launch and no
 // block waits for another.
+// 64 requests of one token each, or 500 with half a million tokens: 17 us a call from Python, most of it on the host.
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxRequests = 16384;   // 12 bytes of shared memory each
 constexpr int kPlanTokensPerBlock = 2048; // 4 tokens per thread

@@ -25,6 +25,9 @@
 // output.  Where some f is not 1 (scales this library did not write) the softmax multiplies the scores of a page's 16-key
 // groups with it, and V is multiplied with it, rounding once more, to f16.
 // Tensor memory (512 columns): S0, S1, O0, O1; P_i overwrites the first half of S_i.
+// Measured (32 / 8 heads of 128, causal): 4 prompts of 4096 tokens 811 us, 678 TFLOP/s; 3 chunks of up to 513 rows over 8704
+// keys 331 us.  Bound by the softmax's chain of latencies, about 4000 clocks per block of 128 keys for both tiles, which the
+// converting warps' instructions share the schedulers with; the products themselves need about half of that.
 #pragma once
 
 constexpr int TM = 128;                 // rows of a tile; BN keys of a block
