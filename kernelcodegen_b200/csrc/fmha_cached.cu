@@ -1086,8 +1086,8 @@ extern "C" int kcg_fmha_cached_workspace(int64_t D, size_t* bytes) {
   if (D != 64 && D != 128) return fail(KCG_ERR_UNSUPPORTED, "fmha_cached: head dimension %lld has no kernel (64, 128)", static_cast<long long>(D));
   const size_t one = split_workspace(D, 1, split_teams(1)), two = split_workspace(D, 2, split_teams(2));
   const size_t many = tiles_workspace(D, sm_count());
-  *bytes = one > two ? one : two;
-  if (many > *bytes) *bytes = many;
+  // The many-row kernel stores its parts 32 bytes at a time, the caller's address is a multiple of 16: 16 bytes to spare.
+  *bytes = std::max({one, two, many}) + 16;
   return KCG_OK;
 }
 
@@ -1129,6 +1129,7 @@ extern "C" int kcg_fmha_cached_fwd(int dtype, int64_t T, int64_t B, int64_t Hq, 
   if (rc) return rc;
   if (!workspace || workspace_bytes < need)
     return fail(KCG_ERR_INVALID_ARG, "fmha_cached: the workspace has %zu bytes, %zu are needed", workspace ? workspace_bytes : 0, need);
+  workspace = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(workspace) + 31) & ~static_cast<uintptr_t>(31));
   CachedParams p{};
   p.Q = Q; p.q_st = q_strides[0]; p.q_sh = q_strides[1];
   p.O = O; p.o_st = o_strides[0]; p.o_sh = o_strides[1];

@@ -1,0 +1,49 @@
+"""Calls of the paged-cache entry points that were once answered wrongly, or by a path that no other test reaches."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from tests.helpers import sync_ok
+from tests.test_cache_gpu import check, make, ops
+
+pytestmark = pytest.mark.gpu
+
+MANY = 10 ** 6          # max_new, taken as all rows of the batch: the tile kernel from 49 rows per key head on
+
+
+def attend_c(c, softmax_scale, causal, max_new, at=0, q=None, out=None):
+    """fmha_cached through the C ABI, with a workspace of exactly the bytes asked for, `at` bytes behind a 512-byte boundary."""
+    from kernelcodegen_b200 import _lib
+    lib = _lib.load()
+    Q, k, v, ks, vs, table, lens = c["args"]
+    Q = Q if q is None else q
+    out = torch.empty_like(Q) if out is None else out
+    strides = lambda t: (ctypes.c_int64 * (t.dim() - 1))(*t.stride()[:-1])  # noqa: E731
+    size = ctypes.c_size_t()
+    assert lib.kcg_fmha_cached_workspace(Q.shape[2], ctypes.byref(size)) == 0
+    room = torch.full((size.value + 1024,), 0x5A, dtype=torch.uint8, device="cuda")
+    room = room[-room.data_ptr() % 512:]
+    _lib.check(lib.kcg_fmha_cached_fwd(_lib.F16 if Q.dtype == torch.float16 else _lib.BF16, Q.shape[0], lens.shape[0], Q.shape[1],
+                                       k.shape[1], Q.shape[2], max_new, softmax_scale, causal, Q.data_ptr(), strides(Q), k.data_ptr(),
+                                       strides(k), ks.data_ptr(), v.data_ptr(), strides(v), vs.data_ptr(), k.shape[0], c["page"],
+                                       table.data_ptr(), table.shape[1], table.stride(0), lens.data_ptr(), c["cu_dev"].data_ptr(),
+                                       out.data_ptr(), strides(out), room.data_ptr() + at, size.value,
+                                       torch.cuda.current_stream().cuda_stream), "kcg_fmha_cached_fwd")
+    sync_ok()
+    assert bool((room[:at] == 0x5A).all()) and bool((room[at + size.value:] == 0x5A).all())
+    return out
+
+
+@pytest.mark.parametrize("at", [0, 16, 32, 48])
+@pytest.mark.parametrize("D", [64, 128])
+def test_workspace_at_any_multiple_of_16_bytes(D, at):
+    """One chunk against a context, in ranges whose parts go through the workspace, and the same by the split kernel."""
+    c = make([2300, 90], [60, 60], 16, 4, 2, D, torch.bfloat16, seed=71)
+    want = ops().fmha_cached(*c["args"], c["cu_dev"], softmax_scale=0.1, causal=True, max_new=60)
+    got = attend_c(c, 0.1, 1, 60, at)
+    check(c, got, 0.1, True, many=True)
+    assert torch.equal(got, want)
+    c = make([2300, 90], [3, 3], 16, 4, 2, D, torch.bfloat16, seed=72)
+    check(c, attend_c(c, 0.1, 1, 3, at), 0.1, True)
