@@ -20,10 +20,11 @@
 // tcgen05 multiplies f16 with f16 or e4m3 with e4m3, not one with the other, and P in e4m3 would keep four bits; so the
 // codes are widened on the way.  Scales: a page's is 2^e f with f in [1, 2).  The power of two, relative to the block's
 // largest (K) or the item's largest so far (V), is multiplied into the codes, exactly where a page lies up to
-// 2^15 below (e4m3's smallest step is 2^-9, f16's 2^-24); further down a code is off by up to 2^-25 of the reference, which
-// beside the reference's own codes is less than the f16 rounding of P.  The references go into the softmax constant and the
-// output.  Where some f is not 1 (scales this library did not write) the softmax multiplies the scores of a page's 16-key
-// groups with it, and V is multiplied with it, rounding once more, to f16.
+// 2^15 below (e4m3's smallest step is 2^-9, f16's 2^-24); further down a code is rounded once, to f16, and off by up to 2^-25
+// of the reference, which beside the reference's own codes is less than the f16 rounding of P.  The references go into the
+// softmax constant and the output.  Where some f is not 1 (scales this library did not write) the softmax multiplies the
+// scores of a page's 16-key groups with it, and V is multiplied with it (and what is left of the power of two) in fp32 and
+// rounded once, to f16.
 // Tensor memory (512 columns): S0, S1, O0, O1; P_i overwrites the first half of S_i.
 // Measured (32 / 8 heads of 128, causal): 4 prompts of 4096 tokens 811 us, 678 TFLOP/s; 3 chunks of up to 513 rows over 8704
 // keys 331 us.  Bound by the softmax's chain of latencies, about 4000 clocks per block of 128 keys for both tiles, which the
@@ -47,9 +48,10 @@ struct BlockRecord {
   int plain;                            // every group's page is there, every f of K is 1
   uint32_t gone;                        // groups whose page is not in the pool: their keys are left out
   int have;                             // keys up to the request's last token; -1: there is no block and none will come
-  int mode[2];                          // of K, V: 0: codes become f16 as they are, 1: times a power of two, 2: there is more to it
-  uint32_t rk[8], rv[8];                // per group of 16 keys: what its codes are multiplied with, two f16
-  float fk[8], fv[8];                   // f
+  int mode[2];                          // of K, V: 0: codes become f16 as they are, 1: times r, 2: there is more to it
+  uint32_t r[2][8];                     // of K, V, per group of 16 keys: what its codes are multiplied with, exactly: two f16
+  float g[2][8];                        // and then, in fp32 with a rounding to f16: what f16 products cannot do
+  float fk[8];                          // f of K, which multiplies the scores
 };
 struct TilesItem {
   int t0, n, len, head, row0;           // the request's first row of Q, rows, keys; key head; first row of the pair
@@ -74,10 +76,8 @@ template <int D> struct TilesSmem {
   int abort;
 };
 
-__device__ __forceinline__ uint32_t f16x2_pow2(int e) {   // 2^e twice, e <= 0, 0 below f16's smallest step
-  const uint32_t h = e >= -14 ? static_cast<uint32_t>(e + 15) << 10 : (e >= -24 ? 1u << (e + 24) : 0u);
-  return h | (h << 16);
-}
+constexpr int kF16MinExp = -14;         // of f16's normal numbers; a code times 2^e, e >= kF16MinExp, is exact in f16
+__device__ __forceinline__ uint32_t f16x2_pow2(int e) { return static_cast<uint32_t>(e + 15) * 0x04000400u; }   // 2^e twice, kF16MinExp <= e <= 0
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23); }
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -654,19 +654,23 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         vexp = max(vexp, vmax);
         const int vnow = vexp == -1000 ? 0 : vexp;
         const float fk = there ? rest(ks_now, ek, kref) : 1.f, fv = there ? rest(vs_now, ev, vnow) : 1.f;
+        // the power of two, relative to the reference: an f16 factor where that is exact, else a part of the fp32 one
+        const int dk = ek == -1000 ? 0 : ek - kref, dv = ev == -1000 ? 0 : ev - vnow;
+        const float gk = dk < kF16MinExp ? pow2f(dk) : 1.f, gv = dv < kF16MinExp ? fv * pow2f(dv) : fv;
         const uint32_t gone = __ballot_sync(0xffffffffu, page == -2);
         const bool plain = __all_sync(0xffffffffu, page != -2 && fk == 1.f);
         const int have = r.len - (block0 + j) * BN;
         const bool full = gone == 0 && have >= BN;
         const bool unit_k = __all_sync(0xffffffffu, !there || ek == kref), unit_v = __all_sync(0xffffffffu, !there || ev == vnow);
-        const bool plain_v = __all_sync(0xffffffffu, fv == 1.f);
+        const bool plain_gk = __all_sync(0xffffffffu, gk == 1.f), plain_gv = __all_sync(0xffffffffu, gv == 1.f);
         if (!mbar_wait(&sm.raw_empty[0], (b & 1u) ^ 1u, abort_flag)) { ok = false; break; }
         BlockRecord& rec = sm.rec[b % RECORDS];
         if (lane < 8) {
-          rec.rk[lane] = f16x2_pow2(ek == -1000 ? 0 : ek - kref);
-          rec.rv[lane] = f16x2_pow2(ev == -1000 ? 0 : ev - vnow);
+          rec.r[0][lane] = f16x2_pow2(dk < kF16MinExp ? 0 : dk);
+          rec.r[1][lane] = f16x2_pow2(dv < kF16MinExp ? 0 : dv);
+          rec.g[0][lane] = gk;
+          rec.g[1][lane] = gv;
           rec.fk[lane] = fk;
-          rec.fv[lane] = fv;
         }
         if (lane == 0) {
           rec.kref = pow2f(kref);
@@ -674,8 +678,8 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
           rec.vshift = j == 0 || vold == vexp ? 1.f : (vold == -1000 ? pow2f(-vexp) : pow2f(vold - vexp));
           rec.plain = plain;
           rec.gone = gone;
-          rec.mode[0] = !full ? 2 : (unit_k ? 0 : 1);
-          rec.mode[1] = !full || !plain_v ? 2 : (unit_v ? 0 : 1);
+          rec.mode[0] = !full || !plain_gk ? 2 : (unit_k ? 0 : 1);
+          rec.mode[1] = !full || !plain_gv ? 2 : (unit_v ? 0 : 1);
           rec.have = go ? min(have, BN) : -1;
         }
         __syncwarp();
@@ -771,23 +775,23 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
                 for (int y = 0; y < 2; ++y) e4m3x4_to_f16(w[x][e][y], h[e][2 * y], h[e][2 * y + 1]);
               if constexpr (kMode > 0) {
-                const uint32_t f = (side ? rec.rv : rec.rk)[r >> 4];
+                const uint32_t f = rec.r[side][r >> 4];
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                   for (int y = 0; y < 4; ++y) h[e][y] = hmul2(h[e][y], f);
               }
               if constexpr (kMode == 2) {
-                const float fv = side ? rec.fv[r >> 4] : 1.f;
+                const float g = rec.g[side][r >> 4];
                 const bool nothing = r >= have || ((gone >> (r >> 4)) & 1u);   // (the bytes may be anything)
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                   for (int y = 0; y < 4; ++y) {
                     uint32_t v = h[e][y];
-                    if (fv != 1.f) {
+                    if (g != 1.f) {
                       const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v));
-                      v = pack_f16(a.x * fv, a.y * fv);
+                      v = pack_f16(a.x * g, a.y * g);
                     }
                     h[e][y] = nothing ? 0u : v;
                   }

@@ -47,3 +47,40 @@ def test_workspace_at_any_multiple_of_16_bytes(D, at):
     assert torch.equal(got, want)
     c = make([2300, 90], [3, 3], 16, 4, 2, D, torch.bfloat16, seed=72)
     check(c, attend_c(c, 0.1, 1, 3, at), 0.1, True)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("big", [0, 9])                  # in a block before most pages, or in a later one
+@pytest.mark.parametrize("below", [14, 15, 20, 25, 28, 33])
+@pytest.mark.parametrize("side", ["K", "V"])
+def test_pages_far_below_their_neighbours_keep_what_f16_holds(side, below, big, causal):
+    """One page's scale is 1, all others 2^-below, and the rows' weight lies on the small ones: a code may be off by half of
+    f16's smallest step, 2^-25 of the largest scale, and not by the code itself."""
+    c = make([200], [64], 16, 4, 2, 64, torch.float16, seed=73, pow2=True)
+    Q = c["Q"].abs()
+    ids = c["table"][0][:13]
+    k, v = (x.clone().float() for x in c["code"])
+    ks, vs = (torch.full_like(x, math.nan) for x in c["scale"])
+    factor = 2.0 ** -below
+    if side == "V":                                       # ordinary keys, but for the big page's, which point away from Q
+        ks[ids], vs[ids] = 2.0 ** -6, factor
+        k[ids[big]], vs[ids[big]] = -448.0, 1.0
+        v[ids] = (v[ids] * 3).clamp(-448, 448)
+        scale = 0.1
+    else:                                                 # a key is +-c in all dims; scores of small pages are of size 5
+        ks[ids], vs[ids] = factor, 2.0 ** -6
+        k[ids] = torch.where(k[ids][..., :1] < 0, -1.0, 1.0) * k[ids][..., :1].abs().clamp(40, 200)
+        k[ids[big]], ks[ids[big]] = -448.0, 1.0
+        scale = 5 / (200 * factor * 51)
+    end = 200 - 12 * 16
+    code = []
+    for x in (k, v):
+        x = x.to(torch.float8_e4m3fn)
+        x.view(torch.uint8)[ids[12], :, end:] = 0x7F
+        code.append(x)
+    c.update(Q=Q, code=code, scale=[ks, vs])
+    c["args"] = (Q.cuda(), code[0].cuda(), code[1].cuda(), ks.cuda(), vs.cuda(), *c["args"][5:])
+    for max_new in (MANY, 1):
+        got = ops().fmha_cached(*c["args"], c["cu_dev"], softmax_scale=scale, causal=causal, max_new=max_new)
+        sync_ok()
+        check(c, got, scale, causal, many=max_new == MANY)
