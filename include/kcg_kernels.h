@@ -603,6 +603,13 @@ KCG_API int kcg_selftest_bounded_wait(uint64_t budget_ns, unsigned long long* wa
                                       void* stream);
 
 /*
+ * Diagnostic: the same for a wait that the 32 lanes of a warp make together.  Half of them run out after
+ * budget_ns (<= 10 ms), the barrier completes after twice that and the other half sees it; the
+ * lanes' answers, a bit each (device memory), must all be the same: 0.
+ */
+KCG_API int kcg_selftest_warp_wait(uint64_t budget_ns, unsigned int* answers_device, void* stream);
+
+/*
  * Row-range owned by one rank when `total` independent units (GEMM rows of A/C,
  * attention batch*head slices, LayerNorm / elementwise rows) are split over
  * `world` GPUs in contiguous blocks rounded to `granule` units.  The reference

@@ -594,11 +594,11 @@ cached_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
   auto meet = [&]() {                       // the team's four warps
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.met);
-    together = mbar_wait(&sm.met, met_parity, &all.abort) && together;
+    together = mbar_wait_warp(&sm.met, met_parity, &all.abort) && together;
     met_parity ^= 1;
   };
   for (int u = 0; u < units; ++u) {
-    if (!mbar_wait(&sm.full[warp][stage], parity, &all.abort)) {
+    if (!mbar_wait_warp(&sm.full[warp][stage], parity, &all.abort)) {
       give_up();
       break;
     }

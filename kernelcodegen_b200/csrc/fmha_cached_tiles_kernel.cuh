@@ -168,10 +168,10 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     prefetch_tmap(&tmV);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&sm.raw_full[s], 1);
-      mbar_init(&sm.raw_empty[s], CONVERT_WARPS);
-      mbar_init(&sm.k_full[s], CONVERT_WARPS);
+      mbar_init(&sm.raw_empty[s], CONVERT_WARPS * 32);
+      mbar_init(&sm.k_full[s], CONVERT_WARPS * 32);
       mbar_init(&sm.k_empty[s], 1);
-      mbar_init(&sm.v_full[s], CONVERT_WARPS);
+      mbar_init(&sm.v_full[s], CONVERT_WARPS * 32);
       mbar_init(&sm.v_empty[s], 1);
       mbar_init(&sm.q_full[s], 4);
       mbar_init(&sm.s_full[s], 1);
@@ -202,6 +202,14 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       if (p.status) *p.status = KCG_ERR_TIMEOUT;
     }
   };
+  // A wait may run out in some lanes of a warp and not in others, and lanes must not leave while others count on them.  Where they do
+  // something together behind a wait they vote on its end; the softmax warps, which a vote per wait would cost time, go on whatever
+  // its end (what they work on is then meaningless, and the status says so) and leave together at the next block's vote, which they
+  // have anyway.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!mbar_wait(bar, parity, abort_flag)) give_up();
+  };
+  auto over = [&]() -> bool { return __any_sync(0xffffffffu, *abort_flag); };
   // ---- this block's range of units ----
   const int per = (p.B + TILES_THREADS - 1) / TILES_THREADS;
   const int i_lo = min(tid * per, p.B), i_hi = min(i_lo + per, p.B);
@@ -319,7 +327,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     bool ok = true, have_q = false;
     float c = 0.f;
     for (uint32_t k_item = 0; ok; ++k_item) {
-      if (!mbar_wait(&sm.item_full[k_item % ITEMS], (k_item / ITEMS) & 1u, abort_flag)) { ok = false; break; }
+      if (!mbar_wait_warp(&sm.item_full[k_item % ITEMS], (k_item / ITEMS) & 1u, abort_flag)) { ok = false; break; }
       const TilesItem& it = sm.item[k_item % ITEMS];
       if (!it.go) break;
       // key blocks of this tile and of the other; keys this row sees from block b on
@@ -339,12 +347,13 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       float m = -INFINITY, l = 0.f, vref = 1.f;
       for (int j = 0; j < n_mine; ++j, ++b, phases ^= 1u) {
         const BlockRecord& rec = sm.rec[b % RECORDS];
-        if (!mbar_wait(&sm.rec_full[b % RECORDS], (b / RECORDS) & 1u, abort_flag)) { ok = false; break; }
+        wait(&sm.rec_full[b % RECORDS], (b / RECORDS) & 1u);
         float cj = c * rec.kref;
-        const bool odd = __any_sync(0xffffffffu, rec.plain == 0 || cj == 0.f);
+        const bool odd = __any_sync(0xffffffffu, rec.plain == 0 || cj == 0.f || *abort_flag);
+        if (odd && over()) { ok = false; break; }
         const float vshift = rec.vshift;
         vref = rec.vref;
-        if (!mbar_wait(&sm.s_full[i], phases & 1u, abort_flag)) { ok = false; break; }
+        wait(&sm.s_full[i], phases & 1u);
         tc_fence_after();
         if (j + 1 == n_mine) {
           // the tile's last scores are there, so its Q is free: the next item's, if that is known already
@@ -390,7 +399,8 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       // The next item's scores may be computed while this one's output leaves.
       if (ok && have_q) c = convert_q();
       if (ok && n_mine > 0) {
-        ok = mbar_wait(&sm.o_full[i], phases >> 1, abort_flag);
+        wait(&sm.o_full[i], phases >> 1);
+        ok = !over();
         phases ^= 2u;
         tc_fence_after();
       }
@@ -440,7 +450,10 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       if (lane == 0) mbar_arrive(&sm.item_empty[k_item % ITEMS]);
       b += max(n_other - n_mine, 0);
     }
-    if (!ok) give_up();
+    if (!ok) {
+      give_up();
+      cp_async_wait_all();                  // queries on their way into this block's memory
+    }
   } else if (warp == 8) {
     // ------------------------------------------------------------------ products
     reg_dealloc<TILES_REGS_OTHER>();
@@ -587,7 +600,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const int take = go ? (p.whole_items ? item_units : min(item_units - block0, units - done)) : 0;
       const int nmax = go ? min(take, in_item - block0) : 1;             // key blocks (none, where the pair sees nothing)
       const bool whole = block0 == 0 && take == item_units;
-      if (!mbar_wait(&sm.item_empty[k_item % ITEMS], ((k_item / ITEMS) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+      if (!mbar_wait_warp(&sm.item_empty[k_item % ITEMS], ((k_item / ITEMS) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
       if (lane == 0) {
         const int slot = k_item == 0 ? 0 : 1;
         sm.item[k_item % ITEMS] = TilesItem{r.t0, r.n, r.len, head, row0, go, block0, max(nmax, 0), whole ? -1 : static_cast<int>(blockIdx.x) * 2 + slot, {0, 0, 0}};
@@ -663,7 +676,11 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const bool full = gone == 0 && have >= BN;
         const bool unit_k = __all_sync(0xffffffffu, !there || ek == kref), unit_v = __all_sync(0xffffffffu, !there || ev == vnow);
         const bool plain_gk = __all_sync(0xffffffffu, gk == 1.f), plain_gv = __all_sync(0xffffffffu, gv == 1.f);
-        if (!mbar_wait(&sm.raw_empty[0], (b & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+        // (with boxes of 32 rows an even group brings the odd one behind it)
+        const bool issue = there && (p.box == 16 || (lane & 1) == 0);
+        const uint32_t bytes = __reduce_add_sync(0xffffffffu, issue ? p.box * D : 0);
+        if (!mbar_wait_warp(&sm.raw_empty[0], (b & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+        if (lane == 0 && go) mbar_expect_tx(&sm.raw_full[0], bytes);
         BlockRecord& rec = sm.rec[b % RECORDS];
         if (lane < 8) {
           rec.r[0][lane] = f16x2_pow2(dk < kF16MinExp ? 0 : dk);
@@ -685,19 +702,13 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.rec_full[b % RECORDS]);
         if (!go) break;
-        // (with boxes of 32 rows an even group brings the odd one behind it)
-        const bool issue = there && (p.box == 16 || (lane & 1) == 0);
-        const uint32_t bytes = __reduce_add_sync(0xffffffffu, issue ? p.box * D : 0);
-#pragma unroll
-        for (int side = 0; side < 2; ++side) {
-          if (side == 1 && !mbar_wait(&sm.raw_empty[1], (b & 1u) ^ 1u, abort_flag)) { ok = false; break; }
-          if (lane == 0) mbar_expect_tx(&sm.raw_full[side], bytes);
-          __syncwarp();
-          if (issue) tma_load_4d(sm.raw[side] + lane * 16 * D, side ? &tmV : &tmK, &sm.raw_full[side], 0, at, head, page);
-        }
-        if (!ok) break;
+        if (issue) tma_load_4d(sm.raw[0] + lane * 16 * D, &tmK, &sm.raw_full[0], 0, at, head, page);
+        if (!mbar_wait_warp(&sm.raw_empty[1], (b & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+        if (lane == 0) mbar_expect_tx(&sm.raw_full[1], bytes);
+        __syncwarp();
+        if (issue) tma_load_4d(sm.raw[1] + lane * 16 * D, &tmV, &sm.raw_full[1], 0, at, head, page);
       }
-      if (!go) break;
+      if (!ok || !go) break;
       blocks += max(nmax, 0);
       if (p.whole_items) {
         next_whole();
@@ -719,8 +730,8 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         }
       }
     }
-    if (!ok) {
-      give_up();
+    if (!ok) give_up();
+    if (over()) {
       int zero = 0;                         // let the copies that were issued land before the block goes away
       for (int s = 0; s < 2; ++s) {
         mbar_wait(&sm.raw_full[s], 0, &zero, 2000000ull);
@@ -806,11 +817,8 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         else if (mode == 1) convert(std::integral_constant<int, 1>{});
         else convert(std::integral_constant<int, 2>{});
         fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&sm.raw_empty[side]);
-          mbar_arrive(side ? &sm.v_full[slot] : &sm.k_full[slot]);
-        }
+        mbar_arrive(&sm.raw_empty[side]);
+        mbar_arrive(side ? &sm.v_full[slot] : &sm.k_full[slot]);
       }
     }
     if (!ok) give_up();

@@ -78,6 +78,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// mbar_wait for all lanes of a warp that do something together afterwards.  Each lane polls with a clock of its own, so when
+// a wait runs out some may still see the barrier complete; the answer is the same in all of them: true if every lane saw it.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                               uint64_t budget_ns = kWaitBudgetNs) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, budget_ns));
+}
+
 // ---- TMA -------------------------------------------------------------------------
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap* m) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");

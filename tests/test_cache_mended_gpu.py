@@ -84,3 +84,15 @@ def test_pages_far_below_their_neighbours_keep_what_f16_holds(side, below, big, 
         got = ops().fmha_cached(*c["args"], c["cu_dev"], softmax_scale=scale, causal=causal, max_new=max_new)
         sync_ok()
         check(c, got, scale, causal, many=max_new == MANY)
+
+
+def test_a_wait_that_runs_out_in_some_lanes_ends_in_all():
+    """What the warps of the attention kernels do together behind a wait needs one answer in all of their lanes."""
+    from kernelcodegen_b200 import _lib
+    lib = _lib.load()
+    answers = torch.full((1,), -1, dtype=torch.int32, device="cuda")
+    assert lib.kcg_selftest_warp_wait(1_000_000, answers.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    sync_ok()
+    assert answers.item() == 0
+    assert lib.kcg_selftest_warp_wait(0, answers.data_ptr(), None) == _lib.ERR_INVALID_ARG
+    assert lib.kcg_selftest_warp_wait(1, None, None) == _lib.ERR_INVALID_ARG
