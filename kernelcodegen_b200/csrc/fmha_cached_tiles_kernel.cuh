@@ -265,10 +265,11 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
     uint32_t b = 0, phases = 0;             // key block; phases of s_full (bit 0) and o_full (bit 1)
     // Rows of Q and O cross global memory whole: PPR lanes with 16 bytes each take a row, RPI rows at a time.
     constexpr int PPR = D / 8, RPI = 32 / PPR;
-    // A thread works out where its own row is (a division) and the others ask it.
-    auto offset_of = [&](const TilesItem& it, int64_t by_token, int64_t by_head) -> int64_t {   // -1: not a row
+    // A thread works out where its own row is (a division) and the others ask it.  (Strides may be negative.)
+    constexpr int64_t NO_ROW = INT64_MIN;
+    auto offset_of = [&](const TilesItem& it, int64_t by_token, int64_t by_head) -> int64_t {
       const int R = it.row0 + i * TM + r;
-      if (R >= it.n * p.G) return -1;
+      if (R >= it.n * p.G) return NO_ROW;
       const int token = R / p.G;
       return (it.t0 + token) * by_token + (it.head * p.G + R - token * p.G) * by_head;
     };
@@ -281,7 +282,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const int64_t at = __shfl_sync(0xffffffffu, mine, k * RPI + lane / PPR);
         const int row = quarter * 32 + k * RPI + lane / PPR, ch = lane % PPR;
         cp_async16(smem_u32(sm.q[i]) + (ch >> 3) * 16384 + row * 128 + (((ch & 7) ^ (row & 7)) << 4),
-                   static_cast<const T*>(p.Q) + max(at, static_cast<int64_t>(0)) + ch * 8, at >= 0);
+                   static_cast<const T*>(p.Q) + (at == NO_ROW ? 0 : at) + ch * 8, at != NO_ROW);
       }
     };
     auto convert_q = [&]() -> float {
@@ -433,7 +434,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             const float f[2] = {__uint_as_float(x[2 * k]) * inv, __uint_as_float(x[2 * k + 1]) * inv};
             reinterpret_cast<uint32_t*>(w)[k] = l == 0.f ? 0u : Words<T>::pack(f);
           }
-          if (at >= 0) {
+          if (at != NO_ROW) {
             uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.O) + at + cc * 32);
             if (p.o_by_32) {                // whole sectors
               st_256(dst, w[0], w[1]);

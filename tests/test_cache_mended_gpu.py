@@ -13,23 +13,26 @@ pytestmark = pytest.mark.gpu
 MANY = 10 ** 6          # max_new, taken as all rows of the batch: the tile kernel from 49 rows per key head on
 
 
-def attend_c(c, softmax_scale, causal, max_new, at=0, q=None, out=None):
-    """fmha_cached through the C ABI, with a workspace of exactly the bytes asked for, `at` bytes behind a 512-byte boundary."""
+def attend_c(c, softmax_scale, causal, max_new, at=0, q=None, out=None, turned=False):
+    """fmha_cached through the C ABI, with a workspace of exactly the bytes asked for, `at` bytes behind a 512-byte boundary.
+    turned: the rows of q and out stand in memory in reverse order, reached by a negative stride."""
     from kernelcodegen_b200 import _lib
     lib = _lib.load()
     Q, k, v, ks, vs, table, lens = c["args"]
     Q = Q if q is None else q
     out = torch.empty_like(Q) if out is None else out
     strides = lambda t: (ctypes.c_int64 * (t.dim() - 1))(*t.stride()[:-1])  # noqa: E731
+    rows = (lambda t: (ctypes.c_int64 * 2)(-t.stride(0), t.stride(1))) if turned else strides  # noqa: E731
+    first = (lambda t: t[-1].data_ptr()) if turned else torch.Tensor.data_ptr  # noqa: E731
     size = ctypes.c_size_t()
     assert lib.kcg_fmha_cached_workspace(Q.shape[2], ctypes.byref(size)) == 0
     room = torch.full((size.value + 1024,), 0x5A, dtype=torch.uint8, device="cuda")
     room = room[-room.data_ptr() % 512:]
     _lib.check(lib.kcg_fmha_cached_fwd(_lib.F16 if Q.dtype == torch.float16 else _lib.BF16, Q.shape[0], lens.shape[0], Q.shape[1],
-                                       k.shape[1], Q.shape[2], max_new, softmax_scale, causal, Q.data_ptr(), strides(Q), k.data_ptr(),
+                                       k.shape[1], Q.shape[2], max_new, softmax_scale, causal, first(Q), rows(Q), k.data_ptr(),
                                        strides(k), ks.data_ptr(), v.data_ptr(), strides(v), vs.data_ptr(), k.shape[0], c["page"],
                                        table.data_ptr(), table.shape[1], table.stride(0), lens.data_ptr(), c["cu_dev"].data_ptr(),
-                                       out.data_ptr(), strides(out), room.data_ptr() + at, size.value,
+                                       first(out), rows(out), room.data_ptr() + at, size.value,
                                        torch.cuda.current_stream().cuda_stream), "kcg_fmha_cached_fwd")
     sync_ok()
     assert bool((room[:at] == 0x5A).all()) and bool((room[at + size.value:] == 0x5A).all())
@@ -96,3 +99,11 @@ def test_a_wait_that_runs_out_in_some_lanes_ends_in_all():
     assert answers.item() == 0
     assert lib.kcg_selftest_warp_wait(0, answers.data_ptr(), None) == _lib.ERR_INVALID_ARG
     assert lib.kcg_selftest_warp_wait(1, None, None) == _lib.ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("B", [1, 160])                  # ranges of key blocks, whole items
+@pytest.mark.parametrize("rows", [2, 60])
+def test_rows_of_q_and_o_in_reverse_order(rows, B):
+    c = make([300] * B, [rows] * B, 16, 4, 2, 64, torch.float16, seed=74)
+    got = attend_c(c, 0.1, 1, rows, q=c["args"][0].flip(0), turned=True)
+    check(c, got.flip(0), 0.1, True, many=rows * 2 > 48)
