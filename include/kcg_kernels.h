@@ -543,6 +543,7 @@ KCG_API int kcg_cache_append(int dtype, int64_t T, int64_t Hkv, int64_t D, const
  * is read behind a request's last token.  Block table entries outside the pool are not followed:
  * their keys are left out, and kcg_device_status() reports KCG_ERR_INVALID_ARG, as it does for
  * lengths beyond the table (cut) and a cu_new that descends or leaves [0, T] (clamped).
+ * At most 2^20 requests.
  * max_new: the most rows a request has, as far as the caller knows (0: T / B is assumed); it chooses the
  * kernel, and a wrong value costs time only.
  *

@@ -44,6 +44,9 @@ namespace {
 using namespace sm100;
 #include "fmha_blocks.cuh"
 
+// The kernels walk the requests one after another, half a microsecond each, while other warps wait for the next that has work, and
+// those waits are limited to two seconds.
+constexpr int kMaxRequests = 1 << 20;
 constexpr int WARPS = 4;            // of a team
 constexpr int WKEYS = 32;           // keys of a warp's tile
 constexpr float kLazy = 14.0f;      // rescale only when the maximum grew by more than 2^14 (p <= 2^14 fits f16)
@@ -1113,7 +1116,8 @@ extern "C" int kcg_fmha_cached_fwd(int dtype, int64_t T, int64_t B, int64_t Hq, 
     return fail(KCG_ERR_INVALID_ARG, "fmha_cached: null pointer");
   if (!cu_new && T % B) return fail(KCG_ERR_INVALID_ARG, "fmha_cached: without cu_new, %lld query rows must divide into %lld requests", static_cast<long long>(T), static_cast<long long>(B));
   if (table_stride < table_width) return fail(KCG_ERR_INVALID_ARG, "fmha_cached: the rows of the block table overlap");
-  if (B > INT32_MAX / 2 || Hq > 65535 || T * Hq > INT32_MAX - 65536 || num_pages > INT32_MAX || table_width > INT32_MAX ||
+  if (B > kMaxRequests) return fail(KCG_ERR_UNSUPPORTED, "fmha_cached: at most %d requests (got %lld)", kMaxRequests, static_cast<long long>(B));
+  if (Hq > 65535 || T * Hq > INT32_MAX - 65536 || num_pages > INT32_MAX || table_width > INT32_MAX ||
       table_width * page_size > INT32_MAX - 65536)
     return fail(KCG_ERR_UNSUPPORTED, "fmha_cached: sizes beyond 32 bits");
   bool ok = aligned16(Q) && aligned16(O) && aligned16(k_cache) && aligned16(v_cache) && aligned16(workspace);

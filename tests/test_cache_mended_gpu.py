@@ -107,3 +107,23 @@ def test_rows_of_q_and_o_in_reverse_order(rows, B):
     c = make([300] * B, [rows] * B, 16, 4, 2, 64, torch.float16, seed=74)
     got = attend_c(c, 0.1, 1, rows, q=c["args"][0].flip(0), turned=True)
     check(c, got.flip(0), 0.1, True, many=rows * 2 > 48)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("rows", [1, 130])
+def test_as_many_requests_as_there_may_be(rows, causal):
+    """The kernels walk past a million requests without queries, from one with work to the next."""
+    B = 2 ** 20
+    c = make([300, 77], [rows, 1], 16, 4, 2, 64, torch.float16, seed=75)
+    at = (5, B - 1)                                       # the two that have work
+    lengths = torch.full((B,), 3, dtype=torch.int32)
+    cu = torch.zeros(B + 1, dtype=torch.int32)
+    cu[at[0] + 1:] = rows
+    cu[B] = rows + 1
+    table = torch.full((B, c["args"][5].shape[1]), -1, dtype=torch.int32, device="cuda")
+    for i, b in enumerate(at):
+        lengths[b] = c["lengths"][i]
+        table[b] = c["args"][5][i]
+    got = ops().fmha_cached(*c["args"][:5], table, lengths.cuda(), cu.cuda(), softmax_scale=0.1, causal=causal, max_new=rows)
+    sync_ok()
+    check(c, got, 0.1, causal, many=rows * 2 > 48)
