@@ -127,3 +127,42 @@ def test_as_many_requests_as_there_may_be(rows, causal):
     got = ops().fmha_cached(*c["args"][:5], table, lengths.cuda(), cu.cuda(), softmax_scale=0.1, causal=causal, max_new=rows)
     sync_ok()
     check(c, got, 0.1, causal, many=rows * 2 > 48)
+
+
+@pytest.mark.parametrize("max_new", [1, 4, MANY])        # 8, 16 rows a tile; 256
+@pytest.mark.parametrize("where", ["key", "key scale", "value", "value scale"])
+@pytest.mark.parametrize("lengths,new,page,Hq,Hkv,D,dtype", [
+    ([200, 90], [60, 1], 16, 4, 2, 128, torch.bfloat16),
+    ([300, 40], [300, 40], 32, 2, 1, 64, torch.float16),                # whole prompts, rows of both tiles
+    ([700, 90] * 3, [400, 90] * 3, 48, 6, 1, 128, torch.float16),       # ranges that end inside an item
+    ([330] * 90, [70] * 90, 16, 4, 2, 64, torch.bfloat16),              # whole items
+])
+def test_what_nan_reaches(lengths, new, page, Hq, Hkv, D, dtype, where, max_new):
+    """A NaN key reaches the rows that see it and no others; a NaN value no other dim, head or request than its own."""
+    c = make(lengths, new, page, Hq, Hkv, D, dtype, seed=76)
+    want = ops().fmha_cached(*c["args"], c["cu_dev"], softmax_scale=0.1, causal=True, max_new=max_new)
+    at = lengths[0] - new[0] // 2                        # a key that half of request 0's rows see
+    p, r = c["table"][0][at // page], at % page
+    k, v, ks, vs = (x.clone() for x in c["args"][1:5])
+    dims = slice(None)
+    if "scale" in where:
+        (ks if where == "key scale" else vs)[p, 0] = math.nan
+        at -= r
+    elif where == "key":
+        k.view(torch.uint8)[p, 0, r, 3] = 0xFF
+    else:
+        v.view(torch.uint8)[p, 0, r, [5, D - 1]] = 0x7F
+        dims = [5, D - 1]
+    got = ops().fmha_cached(c["args"][0], k, v, ks, vs, *c["args"][5:], c["cu_dev"], softmax_scale=0.1, causal=True, max_new=max_new)
+    sync_ok()
+    first = at - (lengths[0] - new[0])                   # the first row that sees it
+    assert 0 < first < new[0]
+    hit, clean = (torch.zeros(want.shape, dtype=torch.bool, device="cuda") for _ in range(2))
+    hit[first:new[0], :Hq // Hkv, dims] = True
+    clean[:] = True                                      # (rows before a NaN value's key may be NaN in its dims, as in a plain product)
+    clean[0 if "value" in where else first:new[0], :Hq // Hkv, dims] = False
+    assert bool(got[hit].isnan().all()) and bool(got[clean].isfinite().all())
+    if "scale" in where:                                 # (other pages' codes may be relative to another scale)
+        check(c, torch.where(clean, got, want), 0.1, True, many=True)
+    else:
+        assert torch.equal(got[clean], want[clean])
