@@ -11,12 +11,12 @@
 //   - The G heads and n_i queries of a key / value head share its keys as the columns of one tile of 8 NQ rows of Q,
 //     so a byte is loaded and converted once.  Products run on mma.sync m16n8k16 with the cache as the 16-row
 //     operand (S^T = K Q^T, O^T = V^T P^T): eight query rows cost no padding, where a tcgen05 tile would want 128.
-//   - Four warps form a team; a team takes four heads of a request side by side (their rows of a token are neighbours in
-//     memory), or two, or one, whose keys the warps then share.  Work is cut in units of 32 keys a warp; the units of the
-//     whole batch, numbered by request, head group, rows and keys, are dealt to a fixed number of teams in equal
-//     contiguous ranges, whatever the lengths: every team finds its range by a prefix sum over the requests.  A team
-//     leaves a partial result (running maximum, sum, output) for at most its first and its last item, which
-//     cached_join_kernel merges in a fixed order.
+//   - Four warps form a team; a team takes two heads of a request side by side (their rows of a token may be neighbours in
+//     memory), or one where the heads do not pair up; two or all four of its warps share a head's keys.  Work is cut in
+//     units of 32 keys a warp; the units of the whole batch, numbered by request, head group, rows and keys, are dealt to a
+//     fixed number of teams in equal contiguous ranges, whatever the lengths: every team finds its range by a prefix sum over
+//     the requests.  A team leaves a partial result (running maximum, sum, output) for at most its first and its last item,
+//     which cached_join_kernel merges in a fixed order.
 //   - A warp of its own feeds each team: it walks the range, looks pages up ahead of use, and fills the warps' rings by
 //     TMA (boxes of 16 or 32 rows of a page), across item borders.  The team's warps know nothing of requests and pages:
 //     a ring entry says what it holds.  They meet only where keys are shared, at the end of an item.
@@ -64,7 +64,7 @@ struct CachedParams {
   const int32_t* cu;                // NULL: `uniform` queries each
   int64_t T, uniform, num_pages;
   int B, Hkv, G, page, causal;
-  int wk_log2;                      // 2^wk_log2 warps share a head's keys, the others take further heads
+  int wk_log2;                      // 2^wk_log2 warps, 2 or 4, share a head's keys; of 2 pairs each has a head of its own
   int whole_items;                  // the many-row kernel: items are dealt whole, not in ranges of key blocks
   int o_by_32;                      // rows of O start on 32-byte boundaries
   int box;                          // rows of a TMA box: 32 where a page is a multiple of that, else 16
@@ -821,28 +821,26 @@ cached_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             o[q][j][x] = o[q][j][x] * mine_w[x & 1] + sm.fold[from][(q * MT + j) * 4 + x][lane] * other_w[x & 1];
       }
     };
-    if (p.wk_log2 > 0) {
-      meet();                      // the fold buffers are free
-      if constexpr (TeamSmem<D, NQ>::FOLDS == 2) {
-        if (p.wk_log2 == 2) {               // 2, 3 into 0, 1
-          if (warp >= 2) give(warp - 2);
-          meet();
-          if (warp < 2) take(warp);
-          meet();
-          if (warp == 1) give(0);
-        } else if (warp & 1) {
-          give(warp >> 1);
-        }
+    meet();                      // the fold buffers are free
+    if constexpr (TeamSmem<D, NQ>::FOLDS == 2) {
+      if (p.wk_log2 == 2) {               // 2, 3 into 0, 1
+        if (warp >= 2) give(warp - 2);
         meet();
-        if (sub == 0) take(warp >> 1);
-      } else {                              // one at a time
-        for (int w = WARPS - 1; w > 0; --w) {
-          if ((w & ((1 << p.wk_log2) - 1)) == 0) continue;
-          if (warp == w) give(0);
-          meet();
-          if (warp == (w >> p.wk_log2) << p.wk_log2) take(0);
-          meet();
-        }
+        if (warp < 2) take(warp);
+        meet();
+        if (warp == 1) give(0);
+      } else if (warp & 1) {
+        give(warp >> 1);
+      }
+      meet();
+      if (sub == 0) take(warp >> 1);
+    } else {                              // one at a time
+      for (int w = WARPS - 1; w > 0; --w) {
+        if ((w & ((1 << p.wk_log2) - 1)) == 0) continue;
+        if (warp == w) give(0);
+        meet();
+        if (warp == (w >> p.wk_log2) << p.wk_log2) take(0);
+        meet();
       }
     }
     if (!together) {
@@ -1037,7 +1035,7 @@ int cache_map(CUtensorMap* tm, const void* cache, const int64_t strides[3], int6
 }
 
 template <typename T, int D, int NQ>
-int launch_split(CachedParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV, int64_t items, void* workspace, cudaStream_t stream) {
+int launch_split(CachedParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV, void* workspace, cudaStream_t stream) {
   const int teams = split_teams(NQ), blocks = sm_count();
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + static_cast<size_t>(teams) * 2 * WARPS * (NQ * D / 4 * 32);
@@ -1067,16 +1065,15 @@ int launch_split(CachedParams& p, const CUtensorMap& tmK, const CUtensorMap& tmV
 
 template <typename T, int D>
 int launch_cached(CachedParams& p, int64_t rows, const CUtensorMap& tmK, const CUtensorMap& tmV, void* workspace, cudaStream_t stream) {
-  const int64_t items = static_cast<int64_t>(p.B) * p.Hkv;
   // Two heads side by side where there are two: as fast as four or one with a head's page in one piece, and 20 % faster
   // than one where a token's heads stand together (8 x 4096 tokens of 32 heads, token-major: 54.8 us, one head 68.2).
   p.wk_log2 = p.Hkv % 2 == 0 ? 1 : 2;
   // Up to 48 rows the split kernel reads the cache once per 16 of them and is still faster than a 256-row item that is
   // mostly empty: 16 requests x 4000 keys x 8 heads, 32 rows 73 against 112 us, 64 rows 125 against 113; 64 x 1000 keys 85
   // against 134 and 148 against 137.
-  if (rows > 48) return launch_tiles<T, D>(p, items * ((rows + 255) / 256), tmK, tmV, workspace, stream);
-  if (rows <= 8) return launch_split<T, D, 1>(p, tmK, tmV, items, workspace, stream);
-  return launch_split<T, D, 2>(p, tmK, tmV, items * ((rows + 15) / 16), workspace, stream);
+  if (rows > 48) return launch_tiles<T, D>(p, static_cast<int64_t>(p.B) * p.Hkv * ((rows + 255) / 256), tmK, tmV, workspace, stream);
+  if (rows <= 8) return launch_split<T, D, 1>(p, tmK, tmV, workspace, stream);
+  return launch_split<T, D, 2>(p, tmK, tmV, workspace, stream);
 }
 
 }  // namespace
