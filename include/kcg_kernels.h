@@ -502,6 +502,10 @@ KCG_API int kcg_layernorm_allgather_multicast(int dtype, int64_t rows, int64_t c
  * kcg_device_status() (KCG_ERR_INVALID_ARG); such a request is not served, the count is clamped.
  * lengths may be cached and free_left may be free_count (update in place); slot_map and
  * block_table overlap nothing.  At most 16384 requests.
+ * A request holds the first ceil(cached[i] / page_size) entries of its row.  Returning pages is the caller's:
+ * all of a request that ends, and, where cached[i] is lowered to `kept` tokens (drafts that were rejected), entries
+ * ceil(kept / page_size) up to the last one it held go back to the end of free_pages before the next plan, which
+ * writes over those entries.
  */
 KCG_API int kcg_cache_plan(int64_t requests, int64_t page_size, int64_t max_tokens,
                            const int32_t* cached, const int32_t* fresh, int32_t* block_table,

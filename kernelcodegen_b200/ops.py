@@ -439,7 +439,20 @@ def cache_plan(cached, new, block_table, free_pages, free_count, page_size: int,
     pages left.  ``out`` may name those four tensors; ``lengths`` may be ``cached`` and ``free_left`` may be
     ``free_count``.  A request that cannot be given all of its pages (or whose tokens end behind max_tokens, or
     whose table row is too short) is left as it was: lengths[i] == cached[i], slots -1.  ``block_table`` may
-    have more rows than there are requests; those behind the last one are not touched."""
+    have more rows than there are requests; those behind the last one are not touched.
+
+    Returning pages is the caller's.  Where a request keeps only ``kept`` of its ``lengths`` tokens (0: it has ended; fewer
+    than it had: drafts were rejected), the entries of its row from ceil(kept / page_size) to the last one it held go
+    back to the end of the list before the next plan, which writes over them.  Without a look at the sizes on the host, with
+    a list that has one entry to spare, its last::
+
+        col = torch.arange(block_table.shape[1], device=kept.device)
+        gone = ((col >= (kept[:, None] + page_size - 1) // page_size) &
+                (col < (lengths[:, None] + page_size - 1) // page_size)).flatten()
+        at = torch.where(gone, gone.cumsum(0) - 1 + free_left, free_pages.shape[0] - 1)
+        free_pages.scatter_(0, at, block_table.flatten())
+        free_left += gone.sum()
+    """
     what = "cache_plan"
     _vector(what, "cached", cached, torch.int32)
     B = cached.shape[0]

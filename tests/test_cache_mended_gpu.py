@@ -7,6 +7,7 @@ import torch
 
 from tests.helpers import sync_ok
 from tests.test_cache_gpu import check, make, ops
+from tests.test_cache_mended_cpu import check_pages, draft_steps, give_back
 
 pytestmark = pytest.mark.gpu
 
@@ -166,3 +167,18 @@ def test_what_nan_reaches(lengths, new, page, Hq, Hkv, D, dtype, where, max_new)
         check(c, torch.where(clean, got, want), 0.1, True, many=True)
     else:
         assert torch.equal(got[clean], want[clean])
+
+
+def test_rejected_drafts_give_their_pages_back():
+    """Plans and returns in turn, nothing read on the host in between."""
+    B, page, pages, width = 5, 16, 400, 110
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    table, free_pages, left, cached = torch.full((B, width), -1, dtype=torch.int32, device="cuda"), i32(list(range(pages)) + [-1]), i32([pages]), i32([0] * B)
+    for new, kept in draft_steps(4):
+        want = (cached + i32(new)).tolist()
+        lengths, _, _, left = ops().cache_plan(cached, i32(new), table, free_pages, left, page, sum(new))
+        assert lengths.tolist() == want
+        cached = i32(kept)
+        give_back(cached, lengths, table, free_pages, left, page)
+        check_pages(kept, table.tolist(), free_pages.tolist(), left.item(), page, pages)
+    sync_ok()
