@@ -551,7 +551,8 @@ KCG_API int kcg_cache_append(int dtype, int64_t T, int64_t Hkv, int64_t D, const
  * lengths beyond the table (cut) and a cu_new that descends or leaves [0, T] (clamped).
  * At most 2^20 requests.
  * max_new: the most rows a request has, as far as the caller knows (0: T / B is assumed); it chooses the
- * kernel, and a wrong value costs time only.
+ * kernel for the whole call.  A wrong value costs time, and the kernels round differently (below); which rows and
+ * keys count does not depend on it.
  *
  * dtype of Q and O: KCG_BF16 or KCG_F16; D in {64, 128}; page_size a multiple of 16; any fp32
  * scales.  Statistics and sums are fp32, P is rounded to fp16.  With more than 48 rows per key head

@@ -182,3 +182,24 @@ def test_rejected_drafts_give_their_pages_back():
         give_back(cached, lengths, table, free_pages, left, page)
         check_pages(kept, table.tolist(), free_pages.tolist(), left.item(), page, pages)
     sync_ok()
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+@pytest.mark.parametrize("max_new", [0, 1, 7, 12, 13, 10 ** 6])
+def test_every_max_new_within_the_bound_of_its_kernel(max_new, pow2):
+    """More rows than the kernel was chosen for, or fewer: each is held to its own arithmetic."""
+    c = make([300, 90, 40], [60, 1, 40], 16, 8, 2, 128, torch.bfloat16, seed=77, pow2=pow2)
+    got = ops().fmha_cached(*c["args"], c["cu_dev"], softmax_scale=0.1, causal=True, max_new=max_new)
+    sync_ok()
+    check(c, got, 0.1, True, many=(max_new or -(-101 // 3)) * 4 > 48)
+
+
+@pytest.mark.parametrize("max_new", [0, 1, 512])
+def test_one_call_with_a_chunk_and_single_tokens(max_new):
+    """A step of a server: 40 requests with one token each, and two prompts in chunks, in one call."""
+    new = [1] * 20 + [512] + [1] * 20 + [77]
+    lengths = [37 * i + 1 for i in range(20)] + [1500] + [61 * i + 5 for i in range(20)] + [77]
+    c = make(lengths, new, 16, 8, 2, 128, torch.bfloat16, seed=78, pow2=True)
+    got = ops().fmha_cached(*c["args"], c["cu_dev"], softmax_scale=128 ** -0.5, causal=True, max_new=max_new)
+    sync_ok()
+    check(c, got, 128 ** -0.5, True, many=(max_new or -(-sum(new) // 42)) * 4 > 48)
