@@ -95,13 +95,16 @@ struct NoHook {
 // exponentials on the ordinary path — and wait_o() before the accumulator is touched for a rescale
 // (it returns false if its wait timed out; the rescale is then skipped and the caller gives up).
 // kEmuMask: which pairs of exponentials take the FMA pipe (0 where a NaN score must stay one); kThreshold: the growth of
-// the maximum, in log2 units, that O is not rescaled for.
-template <typename T, int D, int kEmuMask = KCG_FMHA_EMU_MASK, int kThreshold = static_cast<int>(kRescaleThreshold), typename Arrive,
-          typename Decided = NoHook, typename WaitO = NoHook>
+// the maximum, in log2 units, that O is not rescaled for.  kWide: the maximum may be so large that m + kThreshold is rounded up.
+template <typename T, int D, int kEmuMask = KCG_FMHA_EMU_MASK, int kThreshold = static_cast<int>(kRescaleThreshold), bool kWide = false,
+          typename Arrive, typename Decided = NoHook, typename WaitO = NoHook>
 __device__ __forceinline__ bool softmax_block(uint32_t s_addr, uint32_t o_addr, int j, int limit, float c, float& m,
                                               float& l, int lane, Arrive arrive, Decided decided = Decided(),
                                               WaitO wait_o = WaitO()) {
   bool hooks_ok = true;
+  auto outgrown = [](float top, float old) {
+    return kWide ? top - old > static_cast<float>(kThreshold) : top > old + static_cast<float>(kThreshold);
+  };
   uint32_t sreg[BN];
   tmem_ld64(s_addr, reinterpret_cast<uint32_t(&)[64]>(sreg[0]));
   tmem_ld64(s_addr + 64, reinterpret_cast<uint32_t(&)[64]>(sreg[64]));
@@ -162,7 +165,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_addr, uint32_t o_addr, 
   if (speculate) {
     const float neg_m0 = -m;
     exp_half(0, f2_pack(neg_m0, neg_m0));
-    if (!__any_sync(0xffffffffu, mt > m + static_cast<float>(kThreshold))) {
+    if (!__any_sync(0xffffffffu, outgrown(mt, m))) {
       decided();
       hand_over(0);
       half0_done = true;
@@ -175,7 +178,7 @@ __device__ __forceinline__ bool softmax_block(uint32_t s_addr, uint32_t o_addr, 
   }
   if (!half0_done) {
     bool rescale = false;
-    if ((mt > m + static_cast<float>(kThreshold) || m == -INFINITY) && mt > m) {
+    if ((outgrown(mt, m) || m == -INFINITY) && mt > m) {
       alpha = (m == -INFINITY) ? 0.f : fast_exp2(m - mt);
       rescale = (j > 0);
       m = mt;

@@ -677,7 +677,7 @@ cached_split_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         top[q][e] = fmaxf(fmaxf(s[q][0][e], s[q][0][2 + e]), fmaxf(s[q][1][e], s[q][1][2 + e]));
-        outgrown = outgrown || top[q][e] > m[q][e] + kLazy;
+        outgrown = outgrown || top[q][e] - m[q][e] > kLazy;     // (m + kLazy may round up to a p that f16 does not hold)
       }
     if (__any_sync(0xffffffffu, outgrown)) {
 #pragma unroll

@@ -76,6 +76,10 @@ template <int D> struct TilesSmem {
   int abort;
 };
 
+// A score times its constant less the running maximum m is one fused operation in the softmax, while m is a rounded product: they differ by
+// up to half of m's last place, an exponent of 16 from |m| = 2^28 on.  A score is less than 2^30 (D elements of Q below 2^14, codes
+// up to 448), so with a constant below this one products are less than 2^20; others are rounded, as m is, before the softmax.
+constexpr float kWideFactor = 0.0009765625f;
 constexpr int kF16MinExp = -14;         // of f16's normal numbers; a code times 2^e, e >= kF16MinExp, is exact in f16
 __device__ __forceinline__ uint32_t f16x2_pow2(int e) { return static_cast<uint32_t>(e + 15) * 0x04000400u; }   // 2^e twice, kF16MinExp <= e <= 0
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23); }
@@ -291,34 +295,30 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
       const uint32_t row = smem_u32(sm.q[i]) + r * 128;
       auto piece = [&](int k) { return row + (k >> 3) * 16384 + (((k & 7) ^ (r & 7)) << 4); };
       const bool negative = p.scale_log2 < 0.f;          // the softmax's constant is not negative
-      float factor = 1.f;
-      if (std::is_same<T, __nv_bfloat16>::value || negative) {
-        uint32_t w[PPR][4];
+      uint32_t w[PPR][4];
 #pragma unroll
-        for (int k = 0; k < PPR; ++k) lds128(piece(k), w[k]);
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          uint32_t big = 0;
+      for (int k = 0; k < PPR; ++k) lds128(piece(k), w[k]);
+      uint32_t big = 0;
 #pragma unroll
-          for (int k = 0; k < PPR; ++k)
+      for (int k = 0; k < PPR; ++k)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) big = __vmaxu2(big, w[k][x] & 0x7fff7fffu);
-          big = max(big & 0xffffu, big >> 16);
-          int e = static_cast<int>(big >> 7) - 127 - 13;  // largest element to [2^13, 2^14)
-          e = e < -113 ? -113 : e;
-          const float up = __uint_as_float((static_cast<uint32_t>(127 - e) << 23) | (negative ? 0x80000000u : 0u));
-          factor = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        for (int x = 0; x < 4; ++x) big = __vmaxu2(big, w[k][x] & 0x7fff7fffu);
+      big = max(big & 0xffffu, big >> 16);
+      float top[2];
+      Words<T>::unpack(big, top);
+      int e = static_cast<int>(__float_as_uint(top[0]) >> 23) - 127 - 13;       // largest element to [2^13, 2^14)
+      e = e < -113 ? -113 : e;
+      const float up = __uint_as_float((static_cast<uint32_t>(127 - e) << 23) | (negative ? 0x80000000u : 0u));
+      const float factor = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
-          for (int k = 0; k < PPR; ++k)
+      for (int k = 0; k < PPR; ++k) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) w[k][x] = pack_f16(__uint_as_float(w[k][x] << 16) * up, __uint_as_float(w[k][x] & 0xffff0000u) * up);
-        } else {
-#pragma unroll
-          for (int k = 0; k < PPR; ++k)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) w[k][x] ^= 0x80008000u;
+        for (int x = 0; x < 4; ++x) {
+          float f[2];
+          Words<T>::unpack(w[k][x], f);
+          w[k][x] = pack_f16(f[0] * up, f[1] * up);
         }
-#pragma unroll
-        for (int k = 0; k < PPR; ++k) sts128(piece(k), w[k]);
+        sts128(piece(k), w[k]);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -350,7 +350,8 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         const BlockRecord& rec = sm.rec[b % RECORDS];
         wait(&sm.rec_full[b % RECORDS], (b / RECORDS) & 1u);
         float cj = c * rec.kref;
-        const bool odd = __any_sync(0xffffffffu, rec.plain == 0 || cj == 0.f || *abort_flag);
+        // cj of 0, or so large that a score may be wide (one comparison for both)
+        const bool odd = __any_sync(0xffffffffu, rec.plain == 0 || __float_as_uint(cj) - 1u >= __float_as_uint(kWideFactor) - 1u || *abort_flag);
         if (odd && over()) { ok = false; break; }
         const float vshift = rec.vshift;
         vref = rec.vref;
@@ -367,6 +368,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
         }
         if (odd) {
           // scores that a block-wide constant does not serve are put right in place, in pieces that leave registers alone
+          const bool wide = cj >= kWideFactor;
 #pragma unroll 1
           for (int cc = 0; cc < BN / 32; ++cc) {
             uint32_t x[32];
@@ -374,13 +376,13 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             tmem_wait_ld();
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
-              const float f = cj == 0.f ? 0.f : rec.fk[2 * cc + (k >> 4)];
-              x[k] = (rec.gone >> (2 * cc + (k >> 4))) & 1u ? 0xff800000u : __float_as_uint(__uint_as_float(x[k]) * f);
+              const float f = cj == 0.f ? 0.f : rec.fk[2 * cc + (k >> 4)], y = __fmul_rn(__uint_as_float(x[k]) * f, wide ? cj : 1.f);
+              x[k] = (rec.gone >> (2 * cc + (k >> 4))) & 1u ? 0xff800000u : __float_as_uint(y);
             }
             tmem_st32(s_addr + cc * 32, x);
             tmem_wait_st();
           }
-          if (cj == 0.f) cj = 1.f;                       // (-inf times 0 is not -inf)
+          if (cj == 0.f || wide) cj = 1.f;               // (-inf times 0 is not -inf)
         }
         // the scores being complete means that P V of the block before is, too: O may be changed
         if (j > 0 && vshift != 1.f) {
@@ -395,7 +397,7 @@ cached_tiles_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_consta
             tmem_wait_st();
           }
         }
-        softmax_block<__half, D, 0, static_cast<int>(kLazy)>(s_addr, o_addr, j, seen - j * BN, cj, m, l, lane, [&](int half) { mbar_arrive(&sm.p_full[2 * i + half]); });
+        softmax_block<__half, D, 0, static_cast<int>(kLazy), true>(s_addr, o_addr, j, seen - j * BN, cj, m, l, lane, [&](int half) { mbar_arrive(&sm.p_full[2 * i + half]); });
       }
       // The next item's scores may be computed while this one's output leaves.
       if (ok && have_q) c = convert_q();

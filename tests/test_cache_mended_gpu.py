@@ -5,6 +5,7 @@ import math
 import pytest
 import torch
 
+from tests import cache_reference as R
 from tests.helpers import sync_ok
 from tests.test_cache_gpu import check, make, ops
 from tests.test_cache_mended_cpu import check_pages, draft_steps, give_back
@@ -203,3 +204,29 @@ def test_one_call_with_a_chunk_and_single_tokens(max_new):
     got = ops().fmha_cached(*c["args"], c["cu_dev"], softmax_scale=128 ** -0.5, causal=True, max_new=max_new)
     sync_ok()
     check(c, got, 128 ** -0.5, True, many=(max_new or -(-sum(new) // 42)) * 4 > 48)
+
+
+@pytest.mark.parametrize("max_new", [1, MANY])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("softmax_scale", [2.0 ** 12, 2.0 ** 18, 2.0 ** 21, 2.0 ** 23, -2.0 ** 24, 2.0 ** 26, 2.0 ** 34])
+def test_scores_of_any_size(softmax_scale, dtype, causal, max_new):
+    """Scores of 2^15 to 2^40.  Queries and keys are whole numbers, so that scores are exact and the largest wins by 2^12 at least:
+    a row's result is the value of the key with the largest score."""
+    c = make([700, 300], [60, 60], 16, 4, 2, 64, dtype, seed=79, pow2=True)
+    ids = [p for i in range(2) for p in c["table"][i] if p >= 0]
+    g = torch.Generator().manual_seed(80)
+    k = torch.randint(-8, 9, c["code"][0].shape, generator=g).float()
+    nan = torch.isnan(c["code"][0].float())
+    c["code"][0] = torch.where(nan, math.nan, k).to(torch.float8_e4m3fn)
+    c["scale"][0][ids] = 1.0
+    c["Q"] = torch.randint(-8, 9, c["Q"].shape, generator=g).to(dtype)
+    got = ops().fmha_cached(c["Q"].cuda(), c["code"][0].cuda(), c["args"][2], c["scale"][0].cuda(), *c["args"][4:], c["cu_dev"],
+                            softmax_scale=softmax_scale, causal=causal, max_new=max_new)
+    sync_ok()
+    want, _ = R.attend(c["Q"], c["code"][0].double(), c["scale"][0].double(), c["code"][1].double(), c["scale"][1].double(), c["table"],
+                       c["lengths"], c["cu"], c["page"], softmax_scale, causal)
+    # weights are 0, or equal among keys of equal score; a value is an e4m3 code times a power of two, their mean is rounded to
+    # P's and O's types: (2^-11 + eps / 2) of the largest value, and fp32 sums
+    size = max(float((c["code"][1].double().nan_to_num().amax() * c["scale"][1][p].max())) for p in ids)
+    assert bool(((got.cpu().double() - want).abs() <= (2.0 ** -11 + torch.finfo(dtype).eps) * size).all())
