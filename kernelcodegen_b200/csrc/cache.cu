@@ -26,7 +26,7 @@ namespace {
 // bytes.  Every thread block computes the whole prefix sum into its shared memory (a few loads per
 // thread) and then fills its own share of the tokens and requests, so a step is one launch and no
 // block waits for another.
-// 64 requests of one token each, or 500 with half a million tokens: 17 us a call from Python, most of it on the host.
+// 64 requests of one token each, or 500 with 292379 tokens: 16 us a call from Python, most of it on the host.
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxRequests = 16384;   // 12 bytes of shared memory each
 constexpr int kPlanTokensPerBlock = 2048; // 4 tokens per thread
@@ -165,8 +165,11 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const PlanPara
 // Bound by memory: each 16-bit element is read once and leaves as one byte.  A run stays in registers between
 // finding amax and rounding (up to kVecs 16-byte vectors per lane: 64 rows of D = 128 in a block), with all
 // of its loads in flight at once; longer runs are read twice.  8 prompts of 4096 tokens, 8 heads of 128: 51 us, 0.60 of the
-// copy rate (one warp per run with 32 vectors per lane left six warps on an SM: 83 us).  What is left is latency: slots,
-// old scale and rows are three trips to memory, and five blocks of four warps are in flight on an SM.
+// copy rate (one warp per run with 32 vectors per lane left six warps on an SM: 83 us).  What is left: slots, old scale and rows
+// are three trips to memory that nothing overlaps within a block, five blocks of four warps are in flight on an SM, the 96
+// registers of a thread spill about 50 words of the 16-bit kernels, and warps wait at barriers, for the one that finds the runs
+// and for each other's maxima.  37 chunks of 419 tokens on average, 5 heads of 64: 28 us, where the kernel's share blocks each find
+// the same runs again and 39 % of a warp's time is that barrier.
 constexpr int kVecs = 8;
 constexpr int kAppendWarps = 4;
 

@@ -23,9 +23,9 @@
 //   - Codes become f16 in registers (exact: e4m3 is a subset of f16), bf16 queries too, each row scaled by a power
 //     of two.  K's scale multiplies the scores, V's scale the product of its keys: no operand is rounded again but
 //     P, to f16.
-// Measured (32 query heads of 128): 64 ragged requests of up to 4096 keys, 8 key heads: 63 us, 4.5 TB/s; 2 x 131072 keys, 4
-// key heads: 58 us, 4.6 TB/s; 8 such requests 93 % of the copy rate.  Bound by reading the cache, plus about 10 us per call
-// whatever the size: the prefix sum over the requests, the first fill of the rings, the join.
+// Measured (32 query heads of 128): 64 ragged requests of up to 4096 keys, 8 key heads: 63 us, 4.4 TB/s; 2 x 131072 keys, 4
+// key heads: 58 us, 4.6 TB/s; 8 such requests 178 us, 92 % of the copy rate.  Bound by reading the cache, plus about 10 us per
+// call whatever the size: the prefix sum over the requests, the first fill of the rings, the join.
 #include "common.cuh"
 #include "tcgen05.cuh"
 

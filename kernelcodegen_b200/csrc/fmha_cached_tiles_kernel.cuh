@@ -26,9 +26,13 @@
 // scores of a page's 16-key groups with it, and V is multiplied with it (and what is left of the power of two) in fp32 and
 // rounded once, to f16.
 // Tensor memory (512 columns): S0, S1, O0, O1; P_i overwrites the first half of S_i.
-// Measured (32 / 8 heads of 128, causal): 4 prompts of 4096 tokens 811 us, 678 TFLOP/s; 3 chunks of up to 513 rows over 8704
-// keys 331 us.  Bound by the softmax's chain of latencies, about 4000 clocks per block of 128 keys for both tiles, which the
-// converting warps' instructions share the schedulers with; the products themselves need about half of that.
+// Measured (32 / 8 heads of 128, causal): 4 prompts of 4096 tokens 800 us (750 to 840 from run to run), 690 TFLOP/s; 3 chunks of up
+// to 513 rows over up to 8704 keys 336 us.  A block of 128 keys takes both tiles 3.1 us on the fullest SM of the prompts, whose
+// items are dealt whole and whose neighbours read the same keys, and 4.8 us in the chunks, dealt in ranges (start, parts and join
+// included).  The tensor pipe is busy 36 and 30 % of the time, a scheduler issues in 32 and 27 % of the clocks; a warp's time
+// goes to waits for barriers, tensor memory and loads (31, 34 %), fixed latencies (21, 18 %) and the fetching of instructions (18,
+// 23 %: the roles' code is long, and straight).  The codes have one stage per side, so that a load's latency and the conversion of a
+// block follow one another; where no other SM has just read the keys, as in ranges, that chain is the longer one.
 #pragma once
 
 constexpr int TM = 128;                 // rows of a tile; BN keys of a block
@@ -921,9 +925,12 @@ int launch_tiles(CachedParams& p, int64_t items, const CUtensorMap& tmK, const C
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = p.part_o + static_cast<size_t>(blocks) * 2 * 2 * TM * D;
   p.meta = reinterpret_cast<int*>(p.part_ml + static_cast<size_t>(blocks) * 2 * 2 * TM * 2);
-  // Whole items take as many rounds as the fullest SM has items; ranges of key blocks fill all SMs alike, at about 1.25 times
-  // the cost of a block (no two SMs then work on the same keys at a time) and a tenth of a round for the join.  Measured:
-  // 2048 items 810 whole, 1012 us in ranges; 512 items 128, 183; 128 items 88, 110; 160 items 323, 332; 32 items 636, 197.
+  // Whole items take as many rounds as the fullest SM has items; ranges of key blocks fill all SMs alike, at a block's cost 1.4
+  // times as high (no two SMs then work on the same keys at a time) and a tenth of a round for the join.  Whole items are not
+  // dealt quite evenly under a causal mask (the fullest SM of 2048 has 258 blocks, the average 228), so the calls compare at 1.25.
+  // Measured: 2048 items 810 whole, 1012 us in ranges; 512 items 128, 183; 128 items 88, 110; 160 items 323, 332; 32 items 636, 197.
+  // `items` is what B requests of max_new rows would have: an upper bound, so a call with one long chunk among single tokens
+  // is dealt whole although it has fewer.
   const int64_t rounds = (items + blocks - 1) / blocks;
   p.whole_items = static_cast<double>(rounds) <= 1.25 * static_cast<double>(items) / blocks + 0.1;
   static std::atomic<uint64_t> done{0};
