@@ -544,11 +544,12 @@ KCG_API int kcg_cache_append(int dtype, int64_t T, int64_t Hkv, int64_t D, const
  *   O[j,h,:] = sum_t softmax_t(softmax_scale * Q[j,h,:].K[t,:]) * V[t,:],  t < lengths[i];
  *   causal != 0 masks t > lengths[i] - n + j for the request's j-th of n rows (kcg_fmha_fwd's mask).
  * Rows that see no key are zero; rows of O outside [cu_new[0], cu_new[B]) stay as they were.  Nothing
- * is read behind a request's last token.  A key that is NaN reaches the rows that see it; a value that is
- * NaN, or infinite by its scale, reaches its dim in those and may reach it in rows of the same request and head
- * that come before it (their weight of it is zero, and zero times NaN is NaN, here as in kcg_fmha_fwd).  Block table entries outside the pool are not followed:
- * their keys are left out, and kcg_device_status() reports KCG_ERR_INVALID_ARG, as it does for
- * lengths beyond the table (cut) and a cu_new that descends or leaves [0, T] (clamped).
+ * is read behind a request's last token.  A key that is NaN reaches the rows that see it; a value that
+ * is NaN, or infinite by its scale, reaches its dim in those and may reach it in rows of the same request
+ * and head that come before it (their weight of it is zero, and zero times NaN is NaN, here as in
+ * kcg_fmha_fwd).  Block table entries outside the pool are not followed: their keys are left out, and
+ * kcg_device_status() reports KCG_ERR_INVALID_ARG, as it does for lengths beyond the table (cut) and a
+ * cu_new that descends or leaves [0, T] (clamped).
  * At most 2^20 requests.
  * max_new: the most rows a request has, as far as the caller knows (0: T / B is assumed); it chooses the
  * kernel for the whole call.  A wrong value costs time, and the kernels round differently (below); which rows and

@@ -168,8 +168,8 @@ __global__ void __launch_bounds__(kPlanThreads) cache_plan_kernel(const PlanPara
 // copy rate (one warp per run with 32 vectors per lane left six warps on an SM: 83 us).  What is left: slots, old scale and rows
 // are three trips to memory that nothing overlaps within a block, five blocks of four warps are in flight on an SM, the 96
 // registers of a thread spill about 50 words of the 16-bit kernels, and warps wait at barriers, for the one that finds the runs
-// and for each other's maxima.  37 chunks of 419 tokens on average, 5 heads of 64: 28 us, where the kernel's share blocks each find
-// the same runs again and 39 % of a warp's time is that barrier.
+// and for each other's maxima.  37 chunks of 419 tokens on average, 5 heads of 64: 28 us, where each of the ten blocks that
+// share the heads finds the same runs again and 39 % of a warp's time is spent at barriers.
 constexpr int kVecs = 8;
 constexpr int kAppendWarps = 4;
 
